@@ -11,10 +11,13 @@ from .utils import (_calculate_confidences, convert_to_ms, calculate_confidences
 from .core import PhonemeTimestampAligner  # noqa: F401
 from .inflight import BatchesInFlight  # noqa: F401
 from .windowing import slice_windows, stich_window_predictions, stitch_total_frames  # noqa: F401
+from .rows import (label_loss, label_loss_and_grad, layer_norm, layer_norm_backward, layer_norm_forward,  # noqa: F401
+                   sample_labels)
 from .textgrid import dict_to_textgrid, dict_to_textgrid_with_confidence  # noqa: F401
 
 __all__ = ["AlignmentUtils", "ViterbiDecoder", "_calculate_confidences", "convert_to_ms",
            "calculate_confidences_batch", "log_softmax", "postprocess_batch", "PhonemeTimestampAligner", "BatchesInFlight",
            "slice_windows", "stich_window_predictions", "stitch_total_frames", "dict_to_textgrid",
-           "dict_to_textgrid_with_confidence"]
+           "dict_to_textgrid_with_confidence", "layer_norm", "layer_norm_forward", "layer_norm_backward", "label_loss",
+           "label_loss_and_grad", "sample_labels"]
 __version__ = "0.1.0"

@@ -29,7 +29,11 @@ EXPORTS = ["bfa_version", "bfa_abi_version", "bfa_create", "bfa_destroy", "bfa_l
            "bfa_postprocess", "bfa_log_softmax", "bfa_profile_enable", "bfa_profile_collect",
            "bfa_prepare_emissions", "bfa_stitch_windows", "bfa_align_heads", "bfa_profile_collect_spans", "bfa_set_option",
            "bfa_pack_words", "bfa_pack_results", "bfa_index_records", "bfa_call_path", "bfa_profile_copy",
-           "bfa_pack16_words", "bfa_pack_results16", "bfa_call_counters"]
+           "bfa_pack16_words", "bfa_pack_results16", "bfa_call_counters",
+           "bfa_layer_norm", "bfa_layer_norm_workspace_bytes", "bfa_layer_norm_backward",
+           "bfa_label_loss", "bfa_label_loss_workspace_bytes", "bfa_sample_labels"]
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2  # bfa_rows.dtype
+LOSS_NONE, LOSS_SUM, LOSS_MEAN = 0, 1, 2    # bfa_label_loss
 
 
 class BfaParams(ctypes.Structure):
@@ -54,6 +58,18 @@ class BfaHead(ctypes.Structure):
 class BfaSegment(ctypes.Structure):
     _fields_ = [("phoneme", ctypes.c_int32), ("start", ctypes.c_int32), ("end", ctypes.c_int32),
                 ("target_idx", ctypes.c_int32)]
+
+
+class BfaRows(ctypes.Structure):
+    """include/bfa.h: bfa_rows (the rows [B, T, C] of the row operators)"""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("strideB", ctypes.c_int64), ("strideT", ctypes.c_int64)]
+
+
+class BfaSampleParams(ctypes.Structure):
+    """include/bfa.h: bfa_sample_params"""
+    _fields_ = [("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
+                ("temperature_B", ctypes.c_void_p), ("top_p_B", ctypes.c_void_p), ("min_p_B", ctypes.c_void_p),
+                ("top_k_B", ctypes.c_void_p)]
 
 
 def build(force=False):
@@ -112,6 +128,15 @@ def lib():
     L.bfa_pack_results16.argtypes = [vp, vp, i32, vp, i32, i32, i32, vp, vp]
     L.bfa_call_counters.argtypes = [vp, vp, i32, i32, i32, i32, ctypes.POINTER(BfaParams), ctypes.POINTER(ctypes.c_int32), vp]
     L.bfa_index_records.argtypes = [vp, vp, i32, i64, i32, i32, vp, vp, vp, vp]
+    rows, f32 = ctypes.POINTER(BfaRows), ctypes.c_float
+    L.bfa_layer_norm.argtypes = [vp, rows, i32, i32, i32, vp, vp, vp, i32, f32, rows, vp, vp, vp]
+    L.bfa_layer_norm_workspace_bytes.argtypes = [i32, i32, i32]
+    L.bfa_layer_norm_workspace_bytes.restype = sz
+    L.bfa_layer_norm_backward.argtypes = [vp, rows, rows, i32, i32, i32, vp, vp, i32, vp, vp, rows, vp, vp, vp, sz, vp]
+    L.bfa_label_loss_workspace_bytes.argtypes = [i32, i32, i32]
+    L.bfa_label_loss_workspace_bytes.restype = sz
+    L.bfa_label_loss.argtypes = [vp, rows, i32, i32, i32, vp, vp, vp, i32, f32, vp, vp, rows, vp, sz, vp]
+    L.bfa_sample_labels.argtypes = [vp, rows, i32, i32, i32, vp, vp, ctypes.POINTER(BfaSampleParams), vp, vp, vp]
     _lib = L
     return L
 

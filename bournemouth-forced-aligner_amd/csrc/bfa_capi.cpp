@@ -37,6 +37,18 @@ extern "C" int bfa_launch_pack16(const int32_t *segs, int seg_cap, const int32_t
                                  int32_t *out, void *stream);
 extern "C" int bfa_launch_index_records(const int32_t *rec, int world, int64_t words, int n_max, int n_total, int32_t *owner,
                                         int32_t *offset, int32_t *count, void *stream);
+extern "C" size_t bfa_norm_ws_floats(int B, int T, int C);
+extern "C" int bfa_launch_norm(int dtype, const bfa_rows *x, int B, int T, int C, const int32_t *T_len, const void *w, const void *b,
+                               int wtype, float eps, const bfa_rows *y, float *mean, float *rstd, void *stream);
+extern "C" int bfa_launch_norm_bwd(int dtype, const bfa_rows *dy, const bfa_rows *x, int B, int T, int C, const int32_t *T_len,
+                                   const void *w, int wtype, const float *mean, const float *rstd, const bfa_rows *dx, void *dw,
+                                   void *db, float *part, void *stream);
+extern "C" size_t bfa_loss_ws_doubles();
+extern "C" int bfa_launch_loss(const bfa_rows *z, int B, int T, int C, const int32_t *T_len, const int32_t *labels, const float *weights,
+                               int reduction, float scale, const float *up, float *out, const bfa_rows *dz, double *ws, void *stream);
+extern "C" int bfa_sample_max_c();
+extern "C" int bfa_launch_sample(const bfa_rows *z, int B, int T, int C, const int32_t *T_len, const float *u, const bfa_sample_params *p,
+                                 int32_t *label, float *logp, void *stream);
 extern "C" int bfa_call_path_impl(int B, int C, int Smax, const bfa::DevParams *p);
 extern "C" int bfa_launch_copy(void *dst, const void *src, size_t bytes, void *stream);
 static bool staged_post() { return true; } // k_postconf whenever the shapes fit its LDS budget (the tuple-per-lane kernels otherwise)
@@ -771,6 +783,123 @@ int bfa_stitch_windows(bfa_handle h, const float *window_logits, int B, int NW, 
     const int rc = bfa_launch_stitch(window_logits, B, NW, F, C, weights, total_frames, out, out_strideB, out_strideT, stream);
     if (rc != 0) return fail(h, BFA_ERR_LAUNCH, hipGetErrorString((hipError_t)rc));
     return BFA_OK;
+}
+
+// ---- row operators ---------------------------------------------------------------------------------------------------------
+static const char *bad_rows(const bfa_rows *x, int dtype, bool out, int B, int T, int C)
+{
+    if (!x->data) return "null rows";
+    if (x->dtype != dtype || dtype < BFA_F32 || dtype > BFA_BF16) return "the rows of a call have one type: BFA_F32, BFA_F16 or BFA_BF16";
+    if ((uintptr_t)x->data & (dtype == BFA_F32 ? 3u : 1u)) return "rows must be aligned to their type";
+    const int64_t sB = x->strideB < 0 ? -x->strideB : x->strideB, sT = x->strideT < 0 ? -x->strideT : x->strideT;
+    if (out && ((T > 1 && sT < C) || (B > 1 && sB < C))) return "output rows overlap";
+    return nullptr;
+}
+// what every row operator refuses; *empty: nothing to do
+static const char *bad_shape(int B, int T, int C, bool *empty)
+{
+    if (B < 0 || T < 0 || C < 0) return "negative shape";
+    if ((int64_t)B * T >= (1ll << 31)) return "B * T must be below 2^31";
+    *empty = B == 0 || T == 0 || C == 0;
+    return nullptr;
+}
+#define BFA_REFUSE(cond, msg) do { if (cond) return fail(h, BFA_ERR_INVALID_ARGUMENT, msg); } while (0)
+#define BFA_REFUSE_MSG(expr) do { const char *msg_ = (expr); if (msg_) return fail(h, BFA_ERR_INVALID_ARGUMENT, msg_); } while (0)
+static int launched(bfa_handle h, int rc)
+{
+    return rc == 0 ? BFA_OK : fail(h, BFA_ERR_LAUNCH, hipGetErrorString((hipError_t)rc));
+}
+
+int bfa_layer_norm(bfa_handle h, const bfa_rows *x, int B, int T, int C, const int32_t *T_len, const void *weight, const void *bias,
+                   int wtype, float eps, const bfa_rows *y, float *out_mean, float *out_rstd, void *stream)
+{
+    if (!h) return BFA_ERR_INVALID_ARGUMENT;
+    DeviceGuard guard(h);
+    bool empty;
+    BFA_REFUSE_MSG(bad_shape(B, T, C, &empty));
+    if (empty) return BFA_OK;
+    BFA_REFUSE(!x || !y, "null pointer argument");
+    BFA_REFUSE_MSG(bad_rows(x, x->dtype, false, B, T, C));
+    BFA_REFUSE_MSG(bad_rows(y, x->dtype, true, B, T, C));
+    BFA_REFUSE((weight || bias) && (wtype < BFA_F32 || wtype > BFA_BF16), "wtype must be BFA_F32, BFA_F16 or BFA_BF16");
+    BFA_REFUSE(!(eps >= 0.0f), "eps must not be negative");
+    return launched(h, bfa_launch_norm(x->dtype, x, B, T, C, T_len, weight, bias, wtype, eps, y, out_mean, out_rstd, stream));
+}
+
+size_t bfa_layer_norm_workspace_bytes(int B, int T, int C)
+{
+    if (B <= 0 || T <= 0 || C <= 0 || (int64_t)B * T >= (1ll << 31)) return 0;
+    return bfa_norm_ws_floats(B, T, C) * sizeof(float);
+}
+
+int bfa_layer_norm_backward(bfa_handle h, const bfa_rows *dy, const bfa_rows *x, int B, int T, int C, const int32_t *T_len,
+                            const void *weight, int wtype, const float *mean, const float *rstd, const bfa_rows *dx, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!h) return BFA_ERR_INVALID_ARGUMENT;
+    DeviceGuard guard(h);
+    bool empty;
+    BFA_REFUSE_MSG(bad_shape(B, T, C, &empty));
+    if (empty) return BFA_OK;
+    BFA_REFUSE(!x || !dy || !mean || !rstd, "null pointer argument");
+    BFA_REFUSE_MSG(bad_rows(x, x->dtype, false, B, T, C));
+    BFA_REFUSE_MSG(bad_rows(dy, x->dtype, false, B, T, C));
+    if (dx) BFA_REFUSE_MSG(bad_rows(dx, x->dtype, true, B, T, C));
+    BFA_REFUSE((weight || dweight || dbias) && (wtype < BFA_F32 || wtype > BFA_BF16), "wtype must be BFA_F32, BFA_F16 or BFA_BF16");
+    if (dweight || dbias) {
+        BFA_REFUSE(!workspace || ((uintptr_t)workspace & 7), "the workspace must be there and 8-byte aligned");
+        if (workspace_bytes < bfa_layer_norm_workspace_bytes(B, T, C)) return fail(h, BFA_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
+    }
+    if (!dx && !dweight && !dbias) return BFA_OK;
+    return launched(h, bfa_launch_norm_bwd(x->dtype, dy, x, B, T, C, T_len, weight, wtype, mean, rstd, dx, dweight, dbias,
+                                           (float *)workspace, stream));
+}
+
+size_t bfa_label_loss_workspace_bytes(int B, int T, int C)
+{
+    if (B < 0 || T < 0 || C < 0) return 0;
+    return bfa_loss_ws_doubles() * sizeof(double);
+}
+
+int bfa_label_loss(bfa_handle h, const bfa_rows *logits, int B, int T, int C, const int32_t *T_len, const int32_t *labels,
+                   const float *weights, int reduction, float grad_scale, const float *upstream, float *out_loss,
+                   const bfa_rows *grad, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!h) return BFA_ERR_INVALID_ARGUMENT;
+    DeviceGuard guard(h);
+    bool empty;
+    BFA_REFUSE_MSG(bad_shape(B, T, C, &empty));
+    BFA_REFUSE(reduction < BFA_LOSS_NONE || reduction > BFA_LOSS_MEAN, "reduction must be BFA_LOSS_NONE, BFA_LOSS_SUM or BFA_LOSS_MEAN");
+    if (reduction != BFA_LOSS_NONE && !(empty && !out_loss)) {
+        BFA_REFUSE(!workspace || ((uintptr_t)workspace & 7), "the workspace must be there and 8-byte aligned");
+        if (workspace_bytes < bfa_label_loss_workspace_bytes(B, T, C)) return fail(h, BFA_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
+    }
+    if (empty) {
+        if (reduction == BFA_LOSS_NONE || !out_loss) return BFA_OK;
+        const bfa_rows none = {nullptr, BFA_F32, 0, 0};
+        return launched(h, bfa_launch_loss(&none, 0, 1, 1, nullptr, nullptr, nullptr, BFA_LOSS_SUM, 0.0f, nullptr, out_loss, nullptr,
+                                           (double *)workspace, stream));
+    }
+    BFA_REFUSE(!logits || !labels, "null pointer argument");
+    BFA_REFUSE_MSG(bad_rows(logits, logits->dtype, false, B, T, C));
+    if (grad) BFA_REFUSE_MSG(bad_rows(grad, logits->dtype, true, B, T, C));
+    if (!out_loss && !grad) return BFA_OK;
+    return launched(h, bfa_launch_loss(logits, B, T, C, T_len, labels, weights, reduction, grad_scale, upstream, out_loss, grad,
+                                       (double *)workspace, stream));
+}
+
+int bfa_sample_labels(bfa_handle h, const bfa_rows *logits, int B, int T, int C, const int32_t *T_len, const float *uniform,
+                      const bfa_sample_params *params, int32_t *out_label, float *out_logp, void *stream)
+{
+    if (!h) return BFA_ERR_INVALID_ARGUMENT;
+    DeviceGuard guard(h);
+    bool empty;
+    BFA_REFUSE_MSG(bad_shape(B, T, C, &empty));
+    if (C > bfa_sample_max_c()) return fail(h, BFA_ERR_UNSUPPORTED, "C must be at most 524288");
+    if (empty) return BFA_OK;
+    BFA_REFUSE(!logits || !uniform || !params || !out_label, "null pointer argument");
+    BFA_REFUSE_MSG(bad_rows(logits, logits->dtype, false, B, T, C));
+    return launched(h, bfa_launch_sample(logits, B, T, C, T_len, uniform, params, out_label, out_logp, stream));
 }
 
 } // extern "C"

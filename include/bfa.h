@@ -365,6 +365,70 @@ int bfa_pack_results16(bfa_handle h, const bfa_segment *segs, int seg_cap, const
 int bfa_index_records(bfa_handle h, const int32_t *records, int world, int64_t words, int n_max, int n_total,
                       int32_t *out_owner, int32_t *out_offset, int32_t *out_count, void *stream);
 
+/*
+ * Row operators: what stands next to bfa_log_softmax on the rows [B,T,C] of a model's embeddings and logits -- layer
+ * normalisation, the loss of the logits against the labels an alignment gives (out_frame_phoneme), labels drawn from the logits
+ * -- with the gradients a model is trained by.  Rows are float32, float16 or bfloat16 (every bfa_rows of a call has the same
+ * type); element (b,t,c) is data[b*strideB + t*strideT + c], strides in elements, any alignment that the type allows.  T_len
+ * [B] int32 or NULL: rows t >= T_len[b] are not read, and written as said below.  B * T < 2^31; a call with B, T or C == 0 does
+ * nothing (a loss that is one number is then 0).  Sums and statistics are float32 or wider, in a fixed order (no atomics): the
+ * same call gives the same bits.  These calls keep nothing in the handle but the error text, may be captured into a graph, and
+ * use `workspace` only until the stream has passed them -- calls on different streams need different ones.  Outputs do not overlap
+ * inputs.
+ */
+#define BFA_F32 0
+#define BFA_F16 1
+#define BFA_BF16 2
+typedef struct {
+    void *data;
+    int32_t dtype;
+    int64_t strideB, strideT;
+} bfa_rows;
+
+/* y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(mean((x - mean)^2) + eps).  weight, bias [C] of type wtype, or NULL
+ * (1 and 0); out_mean, out_rstd [B,T] float32 or NULL.  Rows behind T_len: y = mean = rstd = 0. */
+int bfa_layer_norm(bfa_handle h, const bfa_rows *x, int B, int T, int C, const int32_t *T_len, const void *weight, const void *bias,
+                   int wtype, float eps, const bfa_rows *y, float *out_mean, float *out_rstd, void *stream);
+/* The gradients: dx (or NULL) as rows, 0 behind T_len; dweight and dbias [C] of type wtype (or NULL: not computed).  weight as in
+ * the forward call, mean and rstd as it wrote them.  The workspace is needed for dweight / dbias. */
+size_t bfa_layer_norm_workspace_bytes(int B, int T, int C);
+int bfa_layer_norm_backward(bfa_handle h, const bfa_rows *dy, const bfa_rows *x, int B, int T, int C, const int32_t *T_len,
+                            const void *weight, int wtype, const float *mean, const float *rstd, const bfa_rows *dx, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Weighted cross entropy of the rows against labels [B,T] int32 and, in the same pass, its gradient.  A row counts when
+ * t < T_len[b], its label >= 0 and its weight (weights [B,T] float32, NULL: 1) is not 0; other rows give 0.  A label >= C gives NaN
+ * (loss and gradient of that row).
+ *   reduction  BFA_LOSS_NONE: out_loss [B,T] = weight * nll; BFA_LOSS_SUM: their sum, BFA_LOSS_MEAN: that / (sum of the weights),
+ *              0 where the weights sum to 0: one float32
+ *   out_loss   NULL: not wanted;  grad NULL: not wanted
+ *   upstream   device, NULL (1), [B,T] for BFA_LOSS_NONE and one float32 otherwise;  grad = grad_scale * upstream * d loss / d logits
+ * The workspace is not needed for BFA_LOSS_NONE. */
+#define BFA_LOSS_NONE 0
+#define BFA_LOSS_SUM 1
+#define BFA_LOSS_MEAN 2
+size_t bfa_label_loss_workspace_bytes(int B, int T, int C);
+int bfa_label_loss(bfa_handle h, const bfa_rows *logits, int B, int T, int C, const int32_t *T_len, const int32_t *labels,
+                   const float *weights, int reduction, float grad_scale, const float *upstream, float *out_loss,
+                   const bfa_rows *grad, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One label per row, drawn from softmax(logits / temperature) restricted to a prefix of the classes in the order (logit
+ * descending, index ascending): at most top_k of them (<= 0: all), the fewest whose probability within those reaches top_p (>= 1:
+ * all), those with at least min_p of the greatest probability; the first class always stays.  With W the weight that is left,
+ * out_label [B,T] int32 is the lowest index up to which, in index order, more than uniform[b,t] * W is reached (numbers outside [0,1)
+ * count as the nearest inside, NaN as 0), out_logp [B,T] float32 (or NULL) the logarithm of its probability within W.
+ * temperature <= 0 or NaN, top_p <= 0 or NaN, min_p > 1 or NaN: the first class of the order, logarithm 0.  NaN logits count as -inf;
+ * a row without a class above -inf and rows behind T_len give -1 and 0.  The *_B arrays ([B], device) override the numbers where
+ * not NULL.  C <= 524288. */
+typedef struct {
+    float temperature, top_p, min_p;
+    int32_t top_k;
+    const float *temperature_B, *top_p_B, *min_p_B;
+    const int32_t *top_k_B;
+} bfa_sample_params;
+int bfa_sample_labels(bfa_handle h, const bfa_rows *logits, int B, int T, int C, const int32_t *T_len, const float *uniform,
+                      const bfa_sample_params *params, int32_t *out_label, float *out_logp, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
