@@ -50,6 +50,7 @@ extern "C" int bfa_sample_max_c();
 extern "C" int bfa_launch_sample(const bfa_rows *z, int B, int T, int C, const int32_t *T_len, const float *u, const bfa_sample_params *p,
                                  int32_t *label, float *logp, void *stream);
 extern "C" int bfa_call_path_impl(int B, int C, int Smax, const bfa::DevParams *p);
+extern "C" int bfa_launch_fill(void *dst, uint32_t value, size_t words, void *stream);
 extern "C" int bfa_launch_copy(void *dst, const void *src, size_t bytes, void *stream);
 static bool staged_post() { return true; } // k_postconf whenever the shapes fit its LDS budget (the tuple-per-lane kernels otherwise)
 
@@ -257,14 +258,9 @@ void ensure_head_streams(bfa_context *h)
             (void)hipStreamDestroy(h->pair[k]);
             h->pair[k] = nullptr;
         }
-    // The runtime maps the streams of one priority onto a few hardware queues (four by default), and a queue runs its
-    // kernels in order: created like the auxiliary streams, this stream landed on the CALLER's queue and the heads
-    // ran one behind the other (profiles/r03_realtext_timeline_before.txt).  A stream of another priority gets a queue
-    // of its own; the later heads are the narrow ones (group head: C = 17), which fill in beside the phoneme head.
-    // Lowest priority (measured against normal / high: 2.37 vs 2.42 / 2.40 ms one step in flight).
-    int prio_lo = 0, prio_hi = 0;
-    (void)hipDeviceGetStreamPriorityRange(&prio_lo, &prio_hi); // (numerically: lowest priority = largest value)
-    if (hipStreamCreateWithPriority(&h->head_stream, hipStreamNonBlocking, prio_lo) != hipSuccess) h->head_stream = nullptr;
+    // Every stream has the default priority: queues of different priorities are not served reliably side by side on this
+    // hardware (work on them has hung), whatever a queue of its own is worth to the later heads.
+    if (hipStreamCreateWithFlags(&h->head_stream, hipStreamNonBlocking) != hipSuccess) h->head_stream = nullptr;
     if (hipEventCreateWithFlags(&h->head_fork, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags(&h->head_join, hipEventDisableTiming) != hipSuccess) {
         if (h->head_stream) (void)hipStreamDestroy(h->head_stream);
@@ -447,9 +443,9 @@ static int align_impl(bfa_handle h, const float *logp, float *row_stats, int64_t
         // marks the frames beyond an utterance itself: no 8 B x B x Tmax fill ahead of the call (32 MB per head for the
         // 4096 x 1000 batch -- and, on the runtime's default four hardware queues, a fill kernel that sat 0.28 ms behind the
         // other head's K0: profiles/r04_realtext_timeline_q4_before.txt)
-        if (!a.row_stats2 &&
-            hipMemsetAsync(row_stats, 0xFF, (size_t)B * (size_t)Tmax * 2 * sizeof(float), (hipStream_t)stream) != hipSuccess)
-            return fail(h, BFA_ERR_LAUNCH, "memset of row_stats failed");
+        // (a kernel, not a memset: a memset node of a captured call is not replayed reliably)
+        if (!a.row_stats2 && bfa_launch_fill(row_stats, 0xFFFFFFFFu, (size_t)B * (size_t)Tmax * 2, stream) != 0)
+            return fail(h, BFA_ERR_LAUNCH, "filling row_stats failed");
     }
     a.B = B; a.Tmax = Tmax; a.C = C; a.Smax = Smax;
     a.T_len = T_len; a.tokens = tokens; a.S_len = S_len;
@@ -533,13 +529,9 @@ int bfa_align_heads(bfa_handle h, const bfa_head *heads, int n_heads, int B, int
     if (!heads || n_heads <= 0 || n_heads > 8) return fail(h, BFA_ERR_INVALID_ARGUMENT, "bad head list");
     for (int k = 0; k < n_heads; ++k)
         if (!heads[k].logits || !heads[k].out_row_stats) return fail(h, BFA_ERR_INVALID_ARGUMENT, "head without logits / out_row_stats");
-    // Two heads side by side.  Round 3 put the later heads on ONE side stream of the lowest priority (a stream of another
-    // priority gets a hardware queue of its own) and head 0 on the caller's: with the runtime's default four queues the
-    // low-priority queue is not served while the other has workgroups waiting -- head 1's first kernel sat 0.27 ms behind
-    // head 0's K0 (profiles/r04_realtext_timeline_q4_before.txt) and a step took 2.1 ms against 1.7 with eight queues.
-    // Now head k runs on pair[k % 2], two streams of the caller's priority on two different queues; the caller's stream
-    // waits for both: 2.09 -> 1.75 ms one call at a time on four queues.  With several calls in flight (three handles) the
-    // six extra streams collide on the queues and the side stream is the better layout (1.46 against 1.66 ms per step):
+    // Two heads side by side: head k runs on pair[k % 2], two streams of the caller's priority on two different queues; the caller's stream
+    // waits for both.  With several calls in flight (three handles) the six extra streams collide on the queues, and the later
+    // heads share one side stream:
     // BFA_OPT_CALLS_IN_FLIGHT tells which caller this is.
     if (n_heads > 1) ensure_head_streams(h);
     const bool paired = n_heads > 1 && !h->calls_in_flight && h->pair[0] && h->pair[1] && h->head_fork;

@@ -101,7 +101,20 @@ __global__ __launch_bounds__(256) void k_stitch_even(const float *__restrict__ w
     }
 }
 
+__global__ __launch_bounds__(256) void k_fill(uint32_t *dst, uint32_t value, size_t words)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (size_t)gridDim.x * 256) dst[i] = value;
+}
+
 } // namespace bfa
+
+extern "C" int bfa_launch_fill(void *dst, uint32_t value, size_t words, void *stream)
+{
+    if (words == 0) return 0;
+    const size_t wg = (words + 255) / 256;
+    hipLaunchKernelGGL(bfa::k_fill, dim3((unsigned)(wg < 8192 ? wg : 8192)), dim3(256), 0, (hipStream_t)stream, (uint32_t *)dst, value, words);
+    return (int)hipGetLastError();
+}
 
 extern "C" int bfa_launch_stitch(const float *win, int B, int NW, int F, int C, const float *weights, int total_frames,
                                  float *out, int64_t oB, int64_t oT, void *stream_)

@@ -244,10 +244,10 @@ constexpr int WIN_MAX_FRAMES = 1536;
 // phonemes that is about -15 per token after the boost, so past ~64 tokens the -1000 line is usually crossed too.
 // bfa_params.window_max_tokens > 0 overrides this limit (e.g. a large value for posteriors known to be CTC-like).
 constexpr int WIN_MAX_TOKENS = 64;
-// Window backpointers as lane masks written by the scalar unit: the consumer spends one v_cmp per code bit (the result
-// lands in an SGPR pair and leaves through s_store_dwordx4) instead of v_cmp + v_addc into per-lane packed dwords, and K2
-// reads its frame's masks straight from memory (no LDS staging).  (false: the packed-dword form, Rw <= 4 only.)
-constexpr bool WIN_SSTORE = true;
+// Window backpointers as lane masks: one v_cmp per code bit, its 64-bit result gathered into a register by v_writelane and
+// stored 64 dwords at a time; K2 reads its frame's masks straight from memory (no LDS staging).  (false: v_cmp + v_addc into
+// per-lane packed dwords, Rw <= 4 only.)
+constexpr bool WIN_MASKS = true;
 __host__ __device__ inline int win_frames_per_word(int rw) { return rw == 1 ? 16 : (rw == 2 ? 8 : 4); }
 __host__ __device__ inline int win_class_for(int L, int bw, int Ts, int max_frames = WIN_MAX_FRAMES)
 {

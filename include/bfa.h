@@ -266,7 +266,7 @@ int bfa_align_heads(bfa_handle h, const bfa_head *heads, int n_heads, int B, int
  *       (core.py:897-937) -- the heads of a call run on two library streams of the caller's priority, i.e. on two
  *       hardware queues even with the runtime's default of four, and share the machine from the first kernel on.
  *       1: the caller keeps several calls in flight on several handles / streams (BatchesInFlight): head 0 stays on the
- *       caller's stream, the others go to one low-priority side stream -- fewer streams per call, the calls overlap each other.
+ *       caller's stream, the others go to one side stream -- fewer streams per call, the calls overlap each other.
  *   BFA_OPT_WINDOW_ROUTING  1 (default): standard-mode calls on the head widths go by the handle's recent calls.  The fast
  *       sliding window of K1 only stands when an utterance ends above the reference's -1000 sentinel
  *       (forced_alignment.py:23,656-682); posteriors that lose ~1 log-unit per frame end every utterance of ~1000 frames below
