@@ -545,7 +545,7 @@ def test_training_a_head_on_its_alignments(gpu_device):
     au = bfa.AlignmentUtils(blank_id=66, silence_id=0)
     res = au.decode_alignments_device(bfa.log_softmax(z.detach()), torch.from_numpy(np.stack(toks)), lengths, [8] * B)
     res.raise_for_status()
-    labels = res.frame_ph.clone()
+    labels = res.frame_phonemes.clone()
     assert labels.shape == (B, T)
     labels[torch.arange(T, device="cuda")[None] >= torch.tensor(lengths, device="cuda")[:, None]] = -1
     loss = bfa.label_loss(z, labels, lengths=lengths)
