@@ -104,6 +104,11 @@ struct OpMin { template <typename V> static __device__ __forceinline__ V f(V a, 
 template <int CTRL> __device__ __forceinline__ float dpp(float x) { return dpp_f<CTRL>(x); }
 template <int CTRL> __device__ __forceinline__ int dpp(int x) { return dpp_i<CTRL>(x); }
 template <int CTRL> __device__ __forceinline__ double dpp(double x) { return dpp_d<CTRL>(x); }
+template <int CTRL> __device__ __forceinline__ unsigned long long dpp(unsigned long long x)
+{
+    const unsigned lo = (unsigned)dpp_i<CTRL>((int)(unsigned)x), hi = (unsigned)dpp_i<CTRL>((int)(x >> 32));
+    return ((unsigned long long)hi << 32) | lo;
+}
 
 // the reduction over the aligned group of G = 4, 16 or 64 lanes, in every lane of the group.  All lanes of a group are active or none.
 template <int G, typename Op, typename V> __device__ __forceinline__ V group_all(V x)

@@ -226,7 +226,20 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
 }
 
 // ---- long rows: a workgroup of 1024 threads per row -------------------------------------------------------------------------
+// A prefix of the order is found without sorting the row:
+//   k <= SAMPLE_LIST_K: at least k classes are no smaller than the k-th greatest of the 256 maxima of 4 threads each.  One sweep
+//     collects the classes from there up (k = 50: about 56 of them), they are sorted, and the draw is made among them.
+//   otherwise: a histogram of numbers and masses over 2048 ranges of the distance m - z shows the range the prefix ends in, one more
+//     sweep collects that range and sorts it (a range of too many classes is divided by 2048 again).  Masses are whole multiples
+//     of 2^-43 or finer there: integer atomics, whose order does not matter.
+//   ranges that still hold too many (thousands of equal or extreme logits): the border is searched bit by bit, a sweep each.
+// The draw itself adds the kept masses of blocks of 64 vectors in index order.
+// Bound: the float64 exponentials of the histogram and of the draw where k does not bound the prefix, latency for few rows.  One
+// workgroup per CU (with two, 64 registers a thread, the float64 polynomial spills: 604 us instead of 235).
+// 512 rows of 131072 bfloat16 logits with parameters of their own 235 us (searching every border bit by bit: 2878), 8 rows of
+// 32000 float32 ones 49 us (472).
 constexpr int SAMPLE_MAX_C = 1 << 19, SAMPLE_BLOCKS = SAMPLE_MAX_C / (64 * 4);
+constexpr int SAMPLE_LIST = 2048, SAMPLE_LIST_K = 224, SAMPLE_BINS = 2048;
 
 // float order as unsigned order (-0 as +0)
 __device__ __forceinline__ uint32_t key_of(float z)
@@ -240,17 +253,27 @@ template <typename T> struct LongRow {
     static constexpr int VEC = 16 / sizeof(T), BLOCK = 64 * VEC;
     const T *z;
     int C;
-    // f(index, value) for every class, in vectors strided over the workgroup
-    template <typename F> __device__ __forceinline__ void sweep(F &&f) const
+    // f(index, value) for every class, in vectors strided over the workgroup, U of them in flight
+    template <int U, typename F> __device__ __forceinline__ void sweep(F &&f) const
     {
         const int n = C / VEC * VEC;
-        for (int i = threadIdx.x * VEC; i < n; i += 1024 * VEC) {
+        int i = threadIdx.x * VEC;
+        for (; i + (U - 1) * 1024 * VEC < n; i += U * 1024 * VEC) {
+            float v[U][VEC];
+#pragma unroll
+            for (int k = 0; k < U; ++k) load_n<T, VEC>(z + i + k * 1024 * VEC, v[k]);
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f(i + k * 1024 * VEC + j, v[k][j]);
+        }
+        for (; i < n; i += 1024 * VEC) {
             float v[VEC];
             load_n<T, VEC>(z + i, v);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f(i + j, clean(v[j]));
+            for (int j = 0; j < VEC; ++j) f(i + j, v[j]);
         }
-        if (n + (int)threadIdx.x < C) f(n + (int)threadIdx.x, clean((float)z[n + threadIdx.x]));
+        if (n + (int)threadIdx.x < C) f(n + (int)threadIdx.x, (float)z[n + threadIdx.x]);
     }
     // this lane's VEC consecutive classes of block k (BLOCK classes, one wave); -inf behind the row
     __device__ __forceinline__ void block(int k, float (&v)[VEC]) const
@@ -266,26 +289,264 @@ template <typename T> struct LongRow {
     }
 };
 
-template <typename T> __global__ __launch_bounds__(1024) void k_sample_long(SampleArgs a)
+struct LongShared {
+    union { unsigned long long bin[SAMPLE_BINS]; double mass[SAMPLE_BLOCKS]; };
+    union { unsigned count[SAMPLE_BINS]; int tied[SAMPLE_BLOCKS]; };
+    unsigned long long list[SAMPLE_LIST], sorted[SAMPLE_LIST]; // ~key << 32 | index: ascending is the order
+    float top4[256];
+    float f[32];
+    double d[32];
+    unsigned long long u[16];
+    int i[32];
+    int n;                    // length of the list
+    uint32_t kt;              // where a prefix ends: its last key, how many classes of that key it holds ...
+    int ties, all_ties;       // ... and how many there are
+    double S;                 // the prefix's mass
+    int at, front;            // the range it ends in, the number of classes in front of it
+    unsigned long long front_mass, total;
+};
+
+template <typename T> struct LongSampler {
+    using Row = LongRow<T>;
+    LongShared &sh;
+    const Row row;
+    const float m;
+    const double inv_t;
+    int &tf, &td, &ti; // turns of block_all
+
+    __device__ __forceinline__ unsigned long long entry(int i, float z) const { return ((unsigned long long)~key_of(z) << 32) | (unsigned)i; }
+    __device__ __forceinline__ float entry_z(unsigned long long e) const { return value_of(~(uint32_t)(e >> 32)); }
+    __device__ __forceinline__ double entry_w(unsigned long long e) const { return weight(entry_z(e), m, inv_t); }
+
+    // the classes that `take` takes, sorted; -> their number, or more than SAMPLE_LIST (then nothing is sorted)
+    template <typename F> __device__ __forceinline__ int collect(F &&take)
+    {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n = 0;
+        __syncthreads();
+        row.template sweep<4>([&](int i, float z) {
+            if (take(z)) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < SAMPLE_LIST) sh.list[at] = entry(i, z);
+            }
+        });
+        __syncthreads();
+        const int n = sh.n;
+        if (n > SAMPLE_LIST) return n;
+        for (int i = threadIdx.x; i < n; i += 1024) { // (each entry finds its place by itself: no steps to wait for each other)
+            const unsigned long long e = sh.list[i];
+            int place = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) place += sh.list[j] < e ? 1 : 0;
+            sh.sorted[place] = e;
+        }
+        __syncthreads();
+        return n;
+    }
+
+    __device__ __forceinline__ int count_from(uint32_t key)
+    {
+        int n = 0;
+        row.template sweep<2>([&](int, float z) { n += key_of(clean(z)) >= key ? 1 : 0; });
+        return block_all<16, OpAdd>(n, sh.i, ti);
+    }
+    __device__ __forceinline__ double mass_from(uint32_t key)
+    {
+        double M = 0.0;
+        row.template sweep<1>([&](int, float z) { z = clean(z); if (key_of(z) >= key) M += weight(z, m, inv_t); });
+        return block_all<16, OpAdd>(M, sh.d, td);
+    }
+
+    // where the first k classes (k > 0) or the shortest prefix of mass p S (k = 0; S < 0: of the whole row) end -> sh.kt, ties,
+    // all_ties, S; k: at most the number of classes above -inf
+    __device__ __forceinline__ void locate(int k, double p, double S)
+    {
+        const int shift = min(51, 31 + __clz(row.C)); // C 2^shift < 2^63
+        const double up = __builtin_ldexp(1.0, shift), down = __builtin_ldexp(1.0, -shift);
+        const float scale = (float)fmin((double)SAMPLE_BINS / 40.0 * inv_t, 1e37);
+        float base = 0.0f, width = (float)SAMPLE_BINS, fine = 1.0f;
+        int front = 0;
+        unsigned long long front_mass = 0;
+        double target = 0.0;
+        auto place = [&](float z) { return fminf(z == m ? 0.0f : (m - z) * scale, (float)SAMPLE_BINS - 0.5f); }; // decreasing in z
+        bool listed = false;
+        int n = 0;
+        for (int level = 0; level < 2 && !listed; ++level) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < SAMPLE_BINS; i += 1024) { sh.bin[i] = 0; sh.count[i] = 0; }
+            __syncthreads();
+            row.template sweep<1>([&](int, float z) {
+                const float v = place(z);
+                if (z > -__builtin_inff() && v >= base && v < base + width) {
+                    const int b = (int)((v - base) * fine);
+                    atomicAdd(&sh.count[b], 1u);
+                    // 2^52 + w 2^shift: its low bits are the whole number
+                    const double x = __builtin_fma(weight(z, m, inv_t), up, 4503599627370496.0);
+                    atomicAdd(&sh.bin[b], (unsigned long long)__double_as_longlong(x) & 0xfffffffffffffull);
+                }
+            });
+            __syncthreads();
+            // two ranges per thread; prefix over the workgroup
+            const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+            const int c0 = (int)sh.count[2 * t], c1 = (int)sh.count[2 * t + 1];
+            const unsigned long long m0 = sh.bin[2 * t], m1 = sh.bin[2 * t + 1];
+            int cs = group_scan<64>(c0 + c1, lane);
+            unsigned long long ms = group_scan<64>(m0 + m1, lane);
+            if (lane == 63) { sh.i[wave] = cs; sh.u[wave] = ms; }
+            if (t == 0) sh.at = -1;
+            __syncthreads();
+            unsigned long long total = 0;
+            for (int w = 0; w < 16; ++w) {
+                if (w < wave) { cs += sh.i[w]; ms += sh.u[w]; }
+                total += sh.u[w];
+            }
+            if (level == 0) target = p * (S < 0.0 ? (double)total * down : S);
+            cs += front - c0 - c1; // what is in front of this thread's ranges
+            ms += front_mass - m0 - m1;
+            auto ends = [&](int c, unsigned long long M) { return k > 0 ? c >= k : (double)M * down >= target; };
+            if (!ends(cs, ms) && ends(cs + c0 + c1, ms + m0 + m1)) {
+                const bool second = !ends(cs + c0, ms + m0);
+                sh.at = 2 * t + (second ? 1 : 0);
+                sh.front = cs + (second ? c0 : 0);
+                sh.front_mass = ms + (second ? m0 : 0);
+            }
+            __syncthreads();
+            const int at = sh.at;
+            if (at < 0) break; // (k: fewer classes than that; a target of 0)
+            front = sh.front;
+            front_mass = sh.front_mass;
+            const unsigned here = sh.count[at];
+            const bool open = level == 0 && at == SAMPLE_BINS - 1; // everything farther away
+            base += (float)at / fine;
+            width = 1.0f / fine;
+            if (here <= SAMPLE_LIST) {
+                n = collect([&](float z) { const float v = place(z); return z > -__builtin_inff() && v >= base && v < base + width; });
+                listed = true;
+            } else if (open) break;
+            fine *= (float)SAMPLE_BINS;
+        }
+        const double M0 = (double)front_mass * down;
+        if (listed) {
+            if (threadIdx.x < 64) {
+                const int lane = threadIdx.x;
+                double run = M0, mass = M0;
+                int K = 0;
+                for (int i0 = 0; i0 < n; i0 += 64) {
+                    const double w = i0 + lane < n ? entry_w(sh.sorted[i0 + lane]) : 0.0;
+                    const double s = group_scan<64>(w, lane);
+                    const unsigned long long in = __ballot(i0 + lane < n && (k > 0 ? front + i0 + lane < k : run + (s - w) < target));
+                    if (in) { K = i0 + 64 - __clzll((long long)in); mass = run + __shfl(s, 63 - __clzll((long long)in)); }
+                    run += __shfl(s, 63);
+                }
+                if (K < 1) K = 1; // (a target that rounding put in front of the range)
+                const uint32_t key = (uint32_t)(sh.sorted[K - 1] >> 32);
+                int ties = 0, all = 0;
+                for (int i0 = 0; i0 < n; i0 += 64) {
+                    const bool same = i0 + lane < n && (uint32_t)(sh.sorted[i0 + lane] >> 32) == key;
+                    ties += __popcll(__ballot(same && i0 + lane < K));
+                    all += __popcll(__ballot(same));
+                }
+                if (lane == 0) { sh.kt = ~key; sh.ties = ties; sh.all_ties = all; sh.S = mass; }
+            }
+            __syncthreads();
+            return;
+        }
+        // bit by bit: the largest key with at least k classes, or the target's mass, from it up
+        uint32_t key = 0;
+        int ties, all;
+        double mass;
+        if (k > 0) {
+            for (int bit = 31; bit >= 0; --bit)
+                if (count_from(key | (1u << bit)) >= k) key |= 1u << bit;
+            const int above = key == ~0u ? 0 : count_from(key + 1);
+            all = count_from(key) - above;
+            ties = k - above;
+            mass = (key == ~0u ? 0.0 : mass_from(key + 1)) + (double)ties * weight(value_of(key), m, inv_t);
+        } else {
+            for (int bit = 31; bit >= 0; --bit)
+                if (mass_from(key | (1u << bit)) >= target) key |= 1u << bit;
+            const double M = key == ~0u ? 0.0 : mass_from(key + 1);
+            all = count_from(key) - (key == ~0u ? 0 : count_from(key + 1));
+            ties = max(ties_taken(M, weight(value_of(key), m, inv_t), all, target), 1);
+            mass = M;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) { sh.kt = key; sh.ties = ties; sh.all_ties = all; sh.S = mass; }
+        __syncthreads();
+    }
+
+    // the draw among the first k of the n sorted classes (one wave, at most 4 each)
+    __device__ __forceinline__ void draw_listed(int n, const Draw &d, float u, int32_t *label, float *logp)
+    {
+        constexpr int E = (SAMPLE_LIST_K + 63) / 64;
+        const int lane = threadIdx.x, kk = min(n, d.k);
+        unsigned long long e[E];
+        double w[E], in_front[E], S = 0.0;
+#pragma unroll
+        for (int c = 0; c < E; ++c) {
+            const int i = c * 64 + lane;
+            e[c] = i < kk ? sh.sorted[i] : ~0ull;
+            w[c] = i < kk ? entry_w(e[c]) : 0.0;
+            const double s = group_scan<64>(w[c], lane);
+            in_front[c] = S + (s - w[c]);
+            S += __shfl(s, 63);
+        }
+        const double target = d.p * S;
+#pragma unroll
+        for (int c = 0; c < E; ++c)
+            if (!(w[c] >= d.q) || (d.p < 1.0 && !(in_front[c] < target))) w[c] = 0.0;
+        double upto[E] = {}, W = 0.0; // the kept mass up to a class and in all, added in the same order
+#pragma unroll
+        for (int c = 0; c < E; ++c) {
+            unsigned long long some = __ballot(w[c] > 0.0);
+            while (some) {
+                const int from = __ffsll((long long)some) - 1;
+                some &= some - 1;
+                const double wj = __shfl(w[c], from);
+                const uint32_t ij = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)e[c], from);
+                W += wj;
+#pragma unroll
+                for (int q = 0; q < E; ++q) upto[q] += ij <= (uint32_t)e[q] ? wj : 0.0;
+            }
+        }
+        const double goal = target_of(u, W);
+        int first = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int c = 0; c < E; ++c)
+            if (w[c] > 0.0) {
+                const int i = (int)(uint32_t)e[c];
+                if (upto[c] > goal) first = min(first, i);
+                last = max(last, i);
+            }
+        first = group_all<64, OpMin>(first);
+        last = group_all<64, OpMax>(last);
+        const int pick = first != 0x7fffffff ? first : last;
+#pragma unroll
+        for (int c = 0; c < E; ++c)
+            if (w[c] > 0.0 && (int)(uint32_t)e[c] == pick) {
+                *label = pick;
+                if (logp) *logp = logp_of(entry_z(e[c]), m, inv_t, W);
+            }
+    }
+};
+
+template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(SampleArgs a)
 {
     using Row = LongRow<T>;
     constexpr int VEC = Row::VEC, W16 = 16;
-    __shared__ float smf[2 * W16];
-    __shared__ double smd[2 * W16];
-    __shared__ int smi[2 * W16];
-    __shared__ double mass[SAMPLE_BLOCKS];
-    __shared__ int tied[SAMPLE_BLOCKS];
+    __shared__ LongShared sh;
     const float NINF = -__builtin_inff();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int tf = 0, td = 0, ti = 0;
     for (uint32_t r = blockIdx.x; r < a.s.rows; r += gridDim.x) {
         uint32_t b, t;
         a.s.split(r, b, t);
-        float m = NINF;
+        float mine = NINF, m = NINF;
         const Row row = {row_in<T>(a.z, b, t), a.s.C};
+        __syncthreads(); // the shared memory is free again
         if (a.s.held(b, t)) {
-            row.sweep([&](int, float z) { m = fmaxf(m, z); });
-            m = block_all<W16, OpMax>(m, smf, tf);
+            row.template sweep<4>([&](int, float z) { mine = fmaxf(mine, z); }); // (fmaxf passes over NaN)
+            m = block_all<W16, OpMax>(mine, sh.f, tf);
         }
         if (m == NINF) { // (the same for all threads)
             if (threadIdx.x == 0) { a.label[r] = -1; if (a.logp) a.logp[r] = 0.0f; }
@@ -294,76 +555,96 @@ template <typename T> __global__ __launch_bounds__(1024) void k_sample_long(Samp
         const Draw d = draw_of(a, b);
         if (d.greedy) {
             int i = a.s.C;
-            row.sweep([&](int j, float z) { if (z == m) i = min(i, j); });
-            i = block_all<W16, OpMin>(i, smi, ti);
+            row.template sweep<4>([&](int j, float z) { i = z == m ? min(i, j) : i; });
+            i = block_all<W16, OpMin>(i, sh.i, ti);
             if (threadIdx.x == 0) { a.label[r] = i; if (a.logp) a.logp[r] = 0.0f; }
             continue;
         }
-        uint32_t kt = 0; // kept: key > kt, and of the classes at kt the first `ties`
-        int ties = a.s.C;
-        auto count_from = [&](uint32_t key) {
-            int n = 0;
-            row.sweep([&](int, float z) { n += key_of(z) >= key ? 1 : 0; });
-            return block_all<W16, OpAdd>(n, smi, ti);
-        };
-        auto mass_from = [&](uint32_t key) {
-            double M = 0.0;
-            row.sweep([&](int, float z) { if (key_of(z) >= key) M += weight(z, m, d.inv_t); });
-            return block_all<W16, OpAdd>(M, smd, td);
-        };
-        double S = 0.0;
-        if (d.k < a.s.C) { // the largest key with at least k classes from it up, bit by bit
-            for (int bit = 31; bit >= 0; --bit)
-                if (count_from(kt | (1u << bit)) >= d.k) kt |= 1u << bit;
-            ties = d.k - (kt == ~0u ? 0 : count_from(kt + 1));
-            S = (kt == ~0u ? 0.0 : mass_from(kt + 1)) + (double)ties * weight(value_of(kt), m, d.inv_t);
-        } else if (d.p < 1.0) S = mass_from(0);
-        if (d.p < 1.0) { // the largest key with at least the target's mass from it up
-            const double target = d.p * S;
-            uint32_t kp = 0;
-            for (int bit = 31; bit >= 0; --bit)
-                if (mass_from(kp | (1u << bit)) >= target) kp |= 1u << bit;
-            const double M = kp == ~0u ? 0.0 : mass_from(kp + 1);
-            const int c = count_from(kp) - (kp == ~0u ? 0 : count_from(kp + 1));
-            kt = kp;
-            ties = max(ties_taken(M, weight(value_of(kp), m, d.inv_t), c, target), 1);
-        }
-        // the kept mass of every block of BLOCK classes, in index order
-        const int nb = (a.s.C + Row::BLOCK - 1) / Row::BLOCK;
-        __syncthreads();
-        for (int k = wave; k < nb; k += W16) {
-            float z[VEC];
-            int c = 0;
-            row.block(k, z);
+        LongSampler<T> own = {sh, row, m, d.inv_t, tf, td, ti};
+        if (d.k <= SAMPLE_LIST_K) {
+            const float q = group_all<4, OpMax>(mine);
+            if ((lane & 3) == 0) sh.top4[threadIdx.x >> 2] = q;
+            __syncthreads();
+            if (wave == 0) { // the k-th greatest of the 256, bit by bit
+                uint32_t key[4], kt = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) c += key_of(z[j]) == kt ? 1 : 0;
-            c = group_all<64, OpAdd>(c);
-            if (lane == 0) tied[k] = c;
-        }
-        __syncthreads();
-        if (wave == 0) { // exclusive prefix
-            int run = 0;
-            for (int k0 = 0; k0 < nb; k0 += 64) {
-                const int c = k0 + lane < nb ? tied[k0 + lane] : 0;
-                const int s = group_scan<64>(c, lane);
-                if (k0 + lane < nb) tied[k0 + lane] = run + s - c;
-                run += __shfl(s, 63);
+                for (int c = 0; c < 4; ++c) key[c] = key_of(sh.top4[c * 64 + lane]);
+                for (int bit = 31; bit >= 0; --bit) {
+                    const uint32_t x = kt | (1u << bit);
+                    int n = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) n += __popcll(__ballot(key[c] >= x));
+                    if (n >= d.k) kt = x;
+                }
+                if (lane == 0) sh.kt = kt;
+            }
+            __syncthreads();
+            const float from = value_of(sh.kt); // (-inf where fewer groups hold anything)
+            const int n = own.collect([&](float z) { return z >= from && z > NINF; });
+            if (n <= SAMPLE_LIST) {
+                if (wave == 0) own.draw_listed(n, d, a.u[r], a.label + r, a.logp ? a.logp + r : nullptr);
+                continue;
             }
         }
+        uint32_t kt = 0; // kept: key > kt, and of the classes at kt the first `ties`
+        int ties = a.s.C, all_ties = 0;
+        double S = -1.0;
+        if (d.k < a.s.C) {
+            int n = 0;
+            row.template sweep<4>([&](int, float z) { n += z > NINF ? 1 : 0; });
+            n = block_all<W16, OpAdd>(n, sh.i, ti);
+            if (d.k < n) {
+                own.locate(d.k, 0.0, 0.0);
+                kt = sh.kt; ties = sh.ties; all_ties = sh.all_ties; S = sh.S;
+            }
+        }
+        if (d.p < 1.0) {
+            own.locate(0, d.p, S);
+            kt = sh.kt; ties = sh.ties; all_ties = sh.all_ties;
+        }
+        // of classes at kt those in front of every block of BLOCK classes, where not all of them are kept
+        const int nb = (a.s.C + Row::BLOCK - 1) / Row::BLOCK;
+        const bool cut = ties < all_ties;
         __syncthreads();
+        if (cut) {
+            for (int k = wave; k < nb; k += W16) {
+                float z[VEC];
+                int c = 0;
+                row.block(k, z);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) c += key_of(z[j]) == kt ? 1 : 0;
+                c = group_all<64, OpAdd>(c);
+                if (lane == 0) sh.tied[k] = c;
+            }
+            __syncthreads();
+            if (wave == 0) { // exclusive prefix
+                int run = 0;
+                for (int k0 = 0; k0 < nb; k0 += 64) {
+                    const int c = k0 + lane < nb ? sh.tied[k0 + lane] : 0;
+                    const int s = group_scan<64>(c, lane);
+                    if (k0 + lane < nb) sh.tied[k0 + lane] = run + s - c;
+                    run += __shfl(s, 63);
+                }
+            }
+            __syncthreads();
+        }
+        // the kept mass of every block, in index order
         auto kept = [&](int k, float (&z)[VEC], double (&w)[VEC]) {
             row.block(k, z);
             int before = 0;
+            if (cut) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) before += key_of(z[j]) == kt ? 1 : 0;
-            before = tied[k] + group_scan<64>(before, lane) - before;
+                for (int j = 0; j < VEC; ++j) before += key_of(z[j]) == kt ? 1 : 0;
+                before = sh.tied[k] + group_scan<64>(before, lane) - before;
+            }
             double L = 0.0;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 const uint32_t key = key_of(z[j]);
-                bool keep = key > kt;
-                if (key == kt) { keep = before < ties; ++before; }
-                w[j] = keep ? weight(z[j], m, d.inv_t) : 0.0;
+                bool keep = key >= kt;
+                if (cut && key == kt) { keep = before < ties; ++before; }
+                w[j] = 0.0;
+                if (keep) w[j] = weight(z[j], m, d.inv_t);
                 if (!(w[j] >= d.q)) w[j] = 0.0;
                 L += w[j];
             }
@@ -373,13 +654,13 @@ template <typename T> __global__ __launch_bounds__(1024) void k_sample_long(Samp
             float z[VEC];
             double w[VEC];
             const double L = group_all<64, OpAdd>(kept(k, z, w));
-            if (lane == 0) mass[k] = L;
+            if (lane == 0) sh.mass[k] = L;
         }
         __syncthreads();
         if (wave == 0) {
             double W = 0.0;
             for (int k0 = 0; k0 < nb; k0 += 64) {
-                const double s = group_scan<64>(k0 + lane < nb ? mass[k0 + lane] : 0.0, lane);
+                const double s = group_scan<64>(k0 + lane < nb ? sh.mass[k0 + lane] : 0.0, lane);
                 W += __shfl(s, 63);
             }
             const double target = target_of(a.u[r], W);
@@ -387,7 +668,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_sample_long(Samp
             double run = 0.0, before = 0.0, last_before = 0.0;
             int pick = -1, last = 0;
             for (int k0 = 0; k0 < nb && pick < 0; k0 += 64) {
-                const double x = k0 + lane < nb ? mass[k0 + lane] : 0.0;
+                const double x = k0 + lane < nb ? sh.mass[k0 + lane] : 0.0;
                 const double s = group_scan<64>(x, lane);
                 const unsigned long long past = __ballot(run + s > target && x > 0.0), some = __ballot(x > 0.0);
                 const int at = past ? __ffsll((long long)past) - 1 : (some ? 63 - __clzll((long long)some) : 0);
@@ -420,7 +701,6 @@ template <typename T> __global__ __launch_bounds__(1024) void k_sample_long(Samp
                 if (a.logp) a.logp[r] = logp_of(zp, m, d.inv_t, W);
             }
         }
-        __syncthreads(); // mass and tied are free again
     }
 }
 

@@ -576,3 +576,18 @@ def test_refusals_on_the_device(gpu_device):
         bfa.sample_labels(torch.zeros(1, (1 << 19) + 1, device="cuda"), torch.zeros(1, device="cuda"))
     with pytest.raises(ValueError, match="2\\^31"):
         bfa.layer_norm(torch.zeros(1, 1, 1, device="cuda").expand(1 << 16, 1 << 15, 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("prm", [dict(top_k=1), dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=224), dict(top_k=225), dict(top_k=3000, top_p=0.7),
+                                 dict(top_p=0.95, temperature=1.2), dict(top_p=0.05), dict(min_p=0.01), dict(temperature=40.0, top_p=0.5),
+                                 dict(temperature=1e-3, top_p=0.9999), dict()],
+                         ids=lambda p: "-".join(f"{k}{v}" for k, v in p.items()) or "plain")
+def test_sample_labels_of_long_rows(prm, dtype, gpu_device):
+    run_sample(1, 2, 40009, dtype, 101, pitch=40013, **prm)
+
+    def lumps(z):  # thousands of equal values; most of the row masked
+        z[:, 0] = torch.round(z[:, 0])
+        z[:, 1, 50:] = -math.inf
+        return z
+    run_sample(1, 2, 9001, dtype, 102, prep=lumps, **prm)
