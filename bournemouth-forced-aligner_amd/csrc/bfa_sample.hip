@@ -6,8 +6,9 @@
 //   W = mass kept;  label = the lowest i with (kept mass up to and including i) > u W;  logp = x_label - log W
 //
 // Which side of a border between two classes u W falls on, and which class is the last one kept, are decisions: they are the
-// same for every order of the work as long as the masses are good to far more digits than u has (24 bits).  Weights and masses
-// are therefore float64 (a float64 fma issues at the rate of a float32 one here); sums have a fixed order, no atomics.
+// same for every order of the work as long as the masses are good to far more digits than u has (24 bits).  They are made in
+// float64 (a float64 fma issues at the rate of a float32 one here), or in float32 where no border lies within the error of the
+// sums (draw_fast); sums have a fixed order, no atomics on floats.
 #include <algorithm>
 
 #include "bfa_rows.hpp"
@@ -107,8 +108,175 @@ template <int G, typename V> __device__ __forceinline__ V group_scan(V x, int l)
     return x;
 }
 
-// Short rows (C <= 512): G lanes share a row, each holds E consecutive classes.  Bound: the float64 exponentials and, with top-k
-// or top-p, the walk down the distinct values from the top (one maximum over the group per value).
+// A row's draw in float32, by a group of G lanes of E consecutive classes each (z: -inf where a lane has none): false where a
+// border lies within the error of the sums, so that the decision is left to float64.
+//   w = 2^((z - m) log2(e) / T) carries three roundings of its exponent: |x| 3 2^-24 w <= 1.1 2^-24, and the exponential's 2^-23 w;
+//   a sum over the row adds at most 14 more to its terms.  So a sum is off by less than (1.25 C + 20 S) 2^-24, and a difference of a
+//   sum and p S or u W by less than three times that.
+template <int G, int E>
+__device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, float m, const Draw &d, float u, int l, int &label, float &logp)
+{
+    const float NINF = -__builtin_inff();
+    const float rate = (float)(d.inv_t * 1.4426950408889634);
+    if (!(rate > 1e-20f && rate < 1e20f && fabsf(m) < 1e30f)) return false; // (the same for the lanes of a group)
+    float w[E], S = 0.0f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) { w[j] = __builtin_amdgcn_exp2f((z[j] - m) * rate); S += w[j]; }
+    S = group_all<G, OpAdd>(S);
+    const float tol = (1.25f * (float)C + 20.0f * S) * (3.0f / 16777216.0f);
+    float zt = NINF; // kept: z > zt, and of the classes at zt the first `ties`
+    int ties = C;
+    bool cut = false, sure = true;
+    // (the median with +inf is the maximum; fmaxf would first quieten NaN, of which there are none)
+    auto next_below = [&](float v) { // the greatest value under v
+        float x = NINF;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x = __builtin_amdgcn_fmed3f(x, z[j] < v ? z[j] : NINF, __builtin_inff());
+        return group_all<G, OpMax>(x);
+    };
+    auto next_from = [&](float v) { // or at v
+        float x = NINF;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x = __builtin_amdgcn_fmed3f(x, z[j] <= v ? z[j] : NINF, __builtin_inff());
+        return group_all<G, OpMax>(x);
+    };
+    auto count_at = [&](float v) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) c += z[j] == v ? 1 : 0;
+        return group_all<G, OpAdd>(c);
+    };
+    auto mass_above = [&](float v) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) s += z[j] > v ? w[j] : 0.0f;
+        return group_all<G, OpAdd>(s);
+    };
+    if (d.k < C) {
+        float hi = m;
+        int n = 0; // classes above hi
+        if (d.k > 8) { // halve the range of the values a few times before walking down
+            float lo = m;
+#pragma unroll
+            for (int j = 0; j < E; ++j) lo = z[j] > NINF ? fminf(lo, z[j]) : lo;
+            lo = group_all<G, OpMin>(lo);
+            for (int i = 0; i < 6; ++i) {
+                const float mid = 0.5f * (lo + hi);
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j) c += z[j] > mid ? 1 : 0;
+                c = group_all<G, OpAdd>(c);
+                const bool below = c < d.k;
+                n = below ? c : n;
+                hi = below ? mid : hi;
+                lo = below ? lo : mid;
+            }
+        }
+        float v = next_from(hi);
+        while (v > NINF) {
+            const int c = count_at(v);
+            if (n + c >= d.k) {
+                zt = v;
+                ties = d.k - n;
+                cut = ties < c;
+                break;
+            }
+            n += c;
+            v = next_below(v);
+        }
+        if (zt > NINF && d.p < 1.0) S = mass_above(zt) + (float)ties * __builtin_amdgcn_exp2f((zt - m) * rate);
+    }
+    if (d.p < 1.0) {
+        const float p = (float)d.p, target = p * S;
+        float hi = m, M = 0.0f; // mass above hi
+        // classes of weight (1 - p) S / C hold less than what is left out
+        float lo = m + __builtin_amdgcn_logf((1.0f - p) * S / (float)C) / rate;
+        for (int i = 0; i < 7; ++i) {
+            const float mid = 0.5f * (lo + hi), s = mass_above(mid);
+            const bool below = s < target;
+            M = below ? s : M;
+            hi = below ? mid : hi;
+            lo = below ? lo : mid;
+        }
+        float v = next_from(hi);
+        sure = false;
+        while (v > NINF) {
+            const int c = count_at(v);
+            const float wv = __builtin_amdgcn_exp2f((v - m) * rate);
+            if (!(M + (float)c * wv < target)) {
+                const float r = fminf(fmaxf(ceilf((target - M) / wv), 1.0f), (float)c);
+                zt = v;
+                ties = (int)r;
+                cut = ties < c;
+                sure = target - (M + (r - 1.0f) * wv) > tol && (M + r * wv) - target > tol;
+                break;
+            }
+            M += (float)c * wv;
+            v = next_below(v);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) w[j] = z[j] >= zt ? w[j] : 0.0f;
+    if (__any(cut)) {
+        int before = 0; // classes at zt with a lower index
+#pragma unroll
+        for (int j = 0; j < E; ++j) before += (z[j] == zt) ? 1 : 0;
+        before = group_scan<G>(before, l) - before;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool tie = z[j] == zt;
+            w[j] = (tie & (before >= ties)) ? 0.0f : w[j];
+            before += tie ? 1 : 0;
+        }
+    }
+    const float q = (float)d.q;
+    if (q > 0.0f) {
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool top = z[j] == m;
+            near |= !top & (w[j] > 0.0f) & (fabsf(w[j] - q) <= q * 3.0517578125e-5f); // (2^-15 > (3 |x| + 2) 2^-24 up to |x| = 170)
+            w[j] = (top | (w[j] >= q)) ? w[j] : 0.0f;
+        }
+        sure = sure && !near;
+    }
+    float L = 0.0f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) L += w[j];
+    const float incl = group_scan<G>(L, l);
+    const float W = __shfl(incl, G - 1, G), target = u * W;
+    const int base = (threadIdx.x & 63) - l;
+    const unsigned long long group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull)) << base;
+    const unsigned long long past = __ballot(incl > target) & group;
+    if (!past) return false;
+    const int lane = __ffsll((long long)past) - 1;
+    // the class: as many as do not pass the target stand in front of it
+    float run = incl - L, in_front = run, upto = __builtin_inff();
+    int pick = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        run += w[j];
+        const bool under = run <= target;
+        pick += under ? 1 : 0;
+        in_front = under ? run : in_front; // (run only grows)
+        upto = __builtin_amdgcn_fmed3f(under ? __builtin_inff() : run, upto, -__builtin_inff());
+    }
+    float zp = z[0];
+#pragma unroll
+    for (int j = 1; j < E; ++j) zp = pick == j ? z[j] : zp;
+    const bool good = (pick < E) & (upto - target > tol) & (target - in_front > tol);
+    const unsigned long long ok = __ballot(good), bad = __ballot(!sure) & group;
+    if (!((ok >> lane) & 1) || bad) return false;
+    label = __shfl(at + pick, lane);
+    zp = __shfl(zp, lane);
+    logp = (float)(((double)zp - (double)m) * d.inv_t) - __builtin_amdgcn_logf(W) * 0.693147181f;
+    return true;
+}
+
+// Short rows (C <= 512): G lanes share a row, each holds E consecutive classes.  Bound: instructions -- the draw in float32, with
+// the end of a prefix bracketed by halving, and float64 for the rows that float32 leaves undecided (about one in a thousand).
+// 4096 x 1000 rows of 67 float32 logits with top-p 0.83 ms (16 lanes to a row 1.27, everything in float64 and walking down from the
+// top 4.6); 300 x 1500 ragged rows of 17 float16 logits with top-k 24 us (37).
 template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sample_short(SampleArgs a)
 {
     constexpr int RPG = 256 / G;
@@ -116,6 +284,8 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
     const int l = threadIdx.x % G, C = a.s.C;
     const int first = l * E, at = min(first, C - E);
     const bool on = first < C;
+    const bool each = a.p.temperature_B || a.p.top_p_B || a.p.min_p_B || a.p.top_k_B;
+    Draw d = draw_of(a, 0);
     for (uint32_t r = blockIdx.x * RPG + threadIdx.x / G; r < a.s.rows; r += gridDim.x * RPG) {
         uint32_t b, t;
         a.s.split(r, b, t);
@@ -130,13 +300,13 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
                 m = fmaxf(m, z[j]);
             }
             m = group_all<G, OpMax>(m);
-            const Draw d = draw_of(a, b);
+            if (each) d = draw_of(a, b);
             if (m > NINF && d.greedy) {
                 int i = C;
 #pragma unroll
                 for (int j = E - 1; j >= 0; --j) i = (z[j] == m) ? at + j : i;
                 label = group_all<G, OpMin>(i);
-            } else if (m > NINF) {
+            } else if (m > NINF && !draw_fast<G, E>(z, at, C, m, d, a.u[r], l, label, logp)) {
                 double w[E], S = 0.0;
 #pragma unroll
                 for (int j = 0; j < E; ++j) { w[j] = weight(z[j], m, d.inv_t); S += w[j]; }
@@ -709,23 +879,33 @@ template <typename T, int G, int E> static void sample_short(const SampleArgs &a
     const uint32_t grid = std::min<uint32_t>((a.s.rows + 256 / G - 1) / (256 / G), 8192);
     hipLaunchKernelGGL((k_sample_short<T, G, E>), dim3(grid), dim3(256), 0, st, a);
 }
+// the fewest lanes a row fits in with at most 20 classes each: reductions over lanes serve more rows at a time
 template <typename T, int G> static void sample_short_e(const SampleArgs &a, hipStream_t st)
 {
-    switch ((a.s.C + G - 1) / G) {
-    case 1: return sample_short<T, G, 1>(a, st);
-    case 2: return sample_short<T, G, 2>(a, st);
-    case 3: return sample_short<T, G, 3>(a, st);
-    case 4: return sample_short<T, G, 4>(a, st);
-    case 5: return sample_short<T, G, 5>(a, st);
-    case 6: return sample_short<T, G, 6>(a, st);
-    case 7: return sample_short<T, G, 7>(a, st);
-    default: return sample_short<T, G, 8>(a, st);
+    const int e = (a.s.C + G - 1) / G;
+    if constexpr (G == 4) {
+        if (e <= 1) return sample_short<T, G, 1>(a, st);
+        if (e <= 2) return sample_short<T, G, 2>(a, st);
+        if (e <= 3) return sample_short<T, G, 3>(a, st);
+        if (e <= 4) return sample_short<T, G, 4>(a, st);
+        if (e <= 5) return sample_short<T, G, 5>(a, st);
+    }
+    if (e <= 6) return sample_short<T, G, 6>(a, st);
+    if (e <= 7) return sample_short<T, G, 7>(a, st);
+    if constexpr (G == 64) return sample_short<T, G, 8>(a, st);
+    else {
+        if (e <= 8) return sample_short<T, G, 8>(a, st);
+        if (e <= 10) return sample_short<T, G, 10>(a, st);
+        if (e <= 12) return sample_short<T, G, 12>(a, st);
+        if (e <= 14) return sample_short<T, G, 14>(a, st);
+        if (e <= 17) return sample_short<T, G, 17>(a, st);
+        return sample_short<T, G, 20>(a, st);
     }
 }
 template <typename T> static void sample_launch(const SampleArgs &a, hipStream_t st)
 {
-    if (a.s.C <= 32) sample_short_e<T, 4>(a, st);
-    else if (a.s.C <= 128) sample_short_e<T, 16>(a, st);
+    if (a.s.C <= 80) sample_short_e<T, 4>(a, st);
+    else if (a.s.C <= 320) sample_short_e<T, 16>(a, st);
     else if (a.s.C <= 512) sample_short_e<T, 64>(a, st);
     else hipLaunchKernelGGL((k_sample_long<T>), dim3(std::min<uint32_t>(a.s.rows, 1024)), dim3(1024), 0, st, a);
 }
