@@ -54,11 +54,8 @@ __global__ __launch_bounds__(NormGeo<TPR>::WG) void k_norm(NormArgs a)
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         at[v] = min((v * TPR + l) * VEC, C - VEC);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            w[v][j] = a.w ? load_w(a.w, a.wtype, at[v] + j) : 1.0f;
-            b[v][j] = a.b ? load_w(a.b, a.wtype, at[v] + j) : 0.0f;
-        }
+        load_w_n<VEC>(a.w, a.wtype, at[v], 1.0f, w[v]);
+        load_w_n<VEC>(a.b, a.wtype, at[v], 0.0f, b[v]);
     }
     auto own = [&](int v, int j) { return v < NV - 1 || (last < C && at[v] + j >= last); };
     for (uint32_t r = blockIdx.x * Geo::RPG + threadIdx.x / TPR; r < a.s.rows; r += gridDim.x * Geo::RPG) {
@@ -119,11 +116,9 @@ __global__ __launch_bounds__(NormGeo<TPR>::WG) void k_norm_bwd(NormArgs a)
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         at[v] = min((v * TPR + l) * VEC, C - VEC);
+        load_w_n<VEC>(a.w, a.wtype, at[v], 1.0f, w[v]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            w[v][j] = a.w ? load_w(a.w, a.wtype, at[v] + j) : 1.0f;
-            sw[v][j] = sb[v][j] = 0.0f;
-        }
+        for (int j = 0; j < VEC; ++j) sw[v][j] = sb[v][j] = 0.0f;
     }
     auto own = [&](int v, int j) { return v < NV - 1 || (last < C && at[v] + j >= last); };
     for (uint32_t r = blockIdx.x * Geo::RPG + threadIdx.x / TPR; r < a.s.rows; r += gridDim.x * Geo::RPG) {

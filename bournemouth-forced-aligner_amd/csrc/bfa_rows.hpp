@@ -75,6 +75,16 @@ __device__ __forceinline__ float load_w(const void *w, int dtype, int i)
     if (dtype == BFA_F16) return (float)((const _Float16 *)w)[i];
     return (float)((const __bf16 *)w)[i];
 }
+// N of them from i on; no weights: `none`
+template <int N> __device__ __forceinline__ void load_w_n(const void *w, int dtype, int i, float none, float (&f)[N])
+{
+    if (!w) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = none;
+    } else if (dtype == BFA_F32) load_n<float, N>((const float *)w + i, f);
+    else if (dtype == BFA_F16) load_n<_Float16, N>((const _Float16 *)w + i, f);
+    else load_n<__bf16, N>((const __bf16 *)w + i, f);
+}
 __device__ __forceinline__ void store_w(void *w, int dtype, int i, float v)
 {
     if (dtype == BFA_F32) ((float *)w)[i] = v;

@@ -86,6 +86,7 @@ def _ptr(t):
 
 
 def _call(dev):
+    # (the C entries work on their handle's device, whatever the current one is)
     L = _lib.lib()
     return L, _lib.handle(dev.index), torch.cuda.current_stream(dev).cuda_stream
 
@@ -124,10 +125,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, lengths=None, statis
     rstd = torch.empty_like(mean) if statistics else None
     keep, rx = _rows(x.detach(), B, T)
     ry = _lib.BfaRows(y.data_ptr(), rx.dtype, T * C, C)
-    with torch.cuda.device(dev):
-        L, h, stream = _call(dev)
-        rc = L.bfa_layer_norm(h, ctypes.byref(rx), B, T, C, _ptr(lens), _ptr(weight), _ptr(bias), wt, eps, ctypes.byref(ry),
-                              _ptr(mean), _ptr(rstd), stream)
+    L, h, stream = _call(dev)
+    rc = L.bfa_layer_norm(h, ctypes.byref(rx), B, T, C, _ptr(lens), _ptr(weight), _ptr(bias), wt, eps, ctypes.byref(ry),
+                          _ptr(mean), _ptr(rstd), stream)
     _lib.check(rc, h, "bfa_layer_norm")
     return y, mean, rstd
 
@@ -158,13 +158,12 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, lengths=None, param_dt
     kx, rx = _rows(x.detach(), B, T)
     kg, rg = _rows(grad.detach(), B, T)
     rdx = _lib.BfaRows(dx.data_ptr(), rx.dtype, T * C, C) if dx is not None else None
-    with torch.cuda.device(dev):
-        L, h, stream = _call(dev)
-        nbytes = L.bfa_layer_norm_workspace_bytes(B, T, C) if need[1] or need[2] else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        rc = L.bfa_layer_norm_backward(h, ctypes.byref(rg), ctypes.byref(rx), B, T, C, _ptr(lens), _ptr(weight), _DTYPES[pdt],
-                                       _ptr(mean), _ptr(rstd), ctypes.byref(rdx) if rdx is not None else None, _ptr(dw), _ptr(db),
-                                       _ptr(ws), nbytes, stream)
+    L, h, stream = _call(dev)
+    nbytes = L.bfa_layer_norm_workspace_bytes(B, T, C) if need[1] or need[2] else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = L.bfa_layer_norm_backward(h, ctypes.byref(rg), ctypes.byref(rx), B, T, C, _ptr(lens), _ptr(weight), _DTYPES[pdt],
+                                   _ptr(mean), _ptr(rstd), ctypes.byref(rdx) if rdx is not None else None, _ptr(dw), _ptr(db),
+                                   _ptr(ws), nbytes, stream)
     _lib.check(rc, h, "bfa_layer_norm_backward")
     return dx, dw, db
 
@@ -216,12 +215,11 @@ def _loss_call(logits, labels, weights, lens, reduction, want_loss, want_grad, s
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
     keep, rz = _rows(logits.detach(), B, T)
     rg = _lib.BfaRows(grad.data_ptr(), rz.dtype, T * C, C) if want_grad else None
-    with torch.cuda.device(dev):
-        L, h, stream = _call(dev)
-        nbytes = L.bfa_label_loss_workspace_bytes(B, T, C) if red != _lib.LOSS_NONE else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        rc = L.bfa_label_loss(h, ctypes.byref(rz), B, T, C, _ptr(lens), labels.data_ptr(), _ptr(weights), red, scale, _ptr(upstream),
-                              _ptr(loss), ctypes.byref(rg) if want_grad else None, _ptr(ws), nbytes, stream)
+    L, h, stream = _call(dev)
+    nbytes = L.bfa_label_loss_workspace_bytes(B, T, C) if red != _lib.LOSS_NONE else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = L.bfa_label_loss(h, ctypes.byref(rz), B, T, C, _ptr(lens), labels.data_ptr(), _ptr(weights), red, scale, _ptr(upstream),
+                          _ptr(loss), ctypes.byref(rg) if want_grad else None, _ptr(ws), nbytes, stream)
     _lib.check(rc, h, "bfa_label_loss")
     return loss, grad
 
@@ -297,9 +295,8 @@ def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     if C == 0:
         return labels.fill_(-1), logp
     kz, rz = _rows(logits.detach(), B, T)
-    with torch.cuda.device(dev):
-        L, h, stream = _call(dev)
-        rc = L.bfa_sample_labels(h, ctypes.byref(rz), B, T, C, _ptr(lens), uniform.data_ptr(), ctypes.byref(p), labels.data_ptr(),
-                                 logp.data_ptr(), stream)
+    L, h, stream = _call(dev)
+    rc = L.bfa_sample_labels(h, ctypes.byref(rz), B, T, C, _ptr(lens), uniform.data_ptr(), ctypes.byref(p), labels.data_ptr(),
+                             logp.data_ptr(), stream)
     _lib.check(rc, h, "bfa_sample_labels")
     return labels, logp
