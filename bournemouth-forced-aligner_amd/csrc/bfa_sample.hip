@@ -45,32 +45,38 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs &a, uint32_t b)
     return d;
 }
 
+// y r + c with the constant in a pair of scalar registers (left to itself the compiler moves every constant of a polynomial into
+// vector registers first, an instruction each)
+__device__ __forceinline__ double fma_c(double y, double r, double c)
+{
+    double o;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(o) : "v"(y), "v"(r), "s"(c));
+    return o;
+}
 // e^x, x <= 0, to about one unit in the last place: x = n ln 2 + r, |r| <= ln 2 / 2, the Taylor polynomial of degree 12
-// (remainder 0.3466^13 / 13! < 2^-52)
+// (remainder 0.3466^13 / 13! < 2^-52); -inf and NaN give 0
 __device__ __forceinline__ double exp_d(double x)
 {
     const double n = __builtin_rint(x * 1.4426950408889634);
     double r = __builtin_fma(n, -0.69314718055994530942, x);  // ln 2 as a double (the product is not rounded) ...
     r = __builtin_fma(n, -2.3190468138462995584e-17, r);      // ... and what that lacks of ln 2
-    double y = 1.0 / 479001600.0;
-    y = __builtin_fma(y, r, 1.0 / 39916800.0);
-    y = __builtin_fma(y, r, 1.0 / 3628800.0);
-    y = __builtin_fma(y, r, 1.0 / 362880.0);
-    y = __builtin_fma(y, r, 1.0 / 40320.0);
-    y = __builtin_fma(y, r, 1.0 / 5040.0);
-    y = __builtin_fma(y, r, 1.0 / 720.0);
-    y = __builtin_fma(y, r, 1.0 / 120.0);
-    y = __builtin_fma(y, r, 1.0 / 24.0);
-    y = __builtin_fma(y, r, 1.0 / 6.0);
+    double y = fma_c(r, 1.0 / 479001600.0, 1.0 / 39916800.0);
+    y = fma_c(y, r, 1.0 / 3628800.0);
+    y = fma_c(y, r, 1.0 / 362880.0);
+    y = fma_c(y, r, 1.0 / 40320.0);
+    y = fma_c(y, r, 1.0 / 5040.0);
+    y = fma_c(y, r, 1.0 / 720.0);
+    y = fma_c(y, r, 1.0 / 120.0);
+    y = fma_c(y, r, 1.0 / 24.0);
+    y = fma_c(y, r, 1.0 / 6.0);
     y = __builtin_fma(y, r, 0.5);
     y = __builtin_fma(y, r, 1.0);
     y = __builtin_fma(y, r, 1.0);
-    return x > -745.0 ? __builtin_ldexp(y, (int)n) : 0.0; // (-inf too)
+    return x > -745.0 ? __builtin_ldexp(y, (int)n) : 0.0;
 }
 __device__ __forceinline__ double weight(float z, float m, double inv_t)
 {
-    if (z == m) return 1.0;
-    return z == -__builtin_inff() ? 0.0 : exp_d(((double)z - (double)m) * inv_t);
+    return exp_d(z == m ? 0.0 : ((double)z - (double)m) * inv_t); // (both may be +inf)
 }
 __device__ __forceinline__ float clean(float z) { return z == z ? z : -__builtin_inff(); }
 __device__ __forceinline__ double target_of(float u, double W) { const double t = (double)u * W; return t > 0.0 ? t : 0.0; }
