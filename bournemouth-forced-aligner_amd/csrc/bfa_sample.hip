@@ -7,8 +7,8 @@
 //
 // Which side of a border between two classes u W falls on, and which class is the last one kept, are decisions: they are the
 // same for every order of the work as long as the masses are good to far more digits than u has (24 bits).  They are made in
-// float64 (a float64 fma issues at the rate of a float32 one here), or in float32 where no border lies within the error of the
-// sums (draw_fast); sums have a fixed order, no atomics on floats.
+// float64, or in float32 where no border lies within the error of the sums (draw_fast); sums have a fixed order, no atomics on
+// floats.
 #include <algorithm>
 
 #include "bfa_rows.hpp"
@@ -54,10 +54,11 @@ __device__ __forceinline__ double fma_c(double y, double r, double c)
     return o;
 }
 // e^x, x <= 0, to about one unit in the last place: x = n ln 2 + r, |r| <= ln 2 / 2, the Taylor polynomial of degree 12
-// (remainder 0.3466^13 / 13! < 2^-52); -inf and NaN give 0
+// (remainder 0.3466^13 / 13! < 2^-52); -inf and NaN give 0.  The sum with 1.5 2^52 rounds to a whole number and holds it in its low
+// bits.
 __device__ __forceinline__ double exp_d(double x)
 {
-    const double n = __builtin_rint(x * 1.4426950408889634);
+    const double big = 6755399441055744.0, sum = __builtin_fma(x, 1.4426950408889634, big), n = sum - big;
     double r = __builtin_fma(n, -0.69314718055994530942, x);  // ln 2 as a double (the product is not rounded) ...
     r = __builtin_fma(n, -2.3190468138462995584e-17, r);      // ... and what that lacks of ln 2
     double y = fma_c(r, 1.0 / 479001600.0, 1.0 / 39916800.0);
@@ -72,7 +73,7 @@ __device__ __forceinline__ double exp_d(double x)
     y = __builtin_fma(y, r, 0.5);
     y = __builtin_fma(y, r, 1.0);
     y = __builtin_fma(y, r, 1.0);
-    return x > -745.0 ? __builtin_ldexp(y, (int)n) : 0.0;
+    return x > -745.0 ? __builtin_ldexp(y, (int)(uint32_t)__double_as_longlong(sum)) : 0.0;
 }
 __device__ __forceinline__ double weight(float z, float m, double inv_t)
 {
@@ -197,7 +198,7 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
         float hi = m, M = 0.0f; // mass above hi
         // classes of weight (1 - p) S / C hold less than what is left out
         float lo = m + __builtin_amdgcn_logf((1.0f - p) * S / (float)C) / rate;
-        for (int i = 0; i < 7; ++i) {
+        for (int i = 0; i < 9; ++i) {
             const float mid = 0.5f * (lo + hi), s = mass_above(mid);
             const bool below = s < target;
             M = below ? s : M;
@@ -281,15 +282,15 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
 
 // Short rows (C <= 512): G lanes share a row, each holds E consecutive classes.  Bound: instructions -- the draw in float32, with
 // the end of a prefix bracketed by halving, and float64 for the rows that float32 leaves undecided (about one in a thousand).
-// 4096 x 1000 rows of 67 float32 logits with top-p 0.83 ms (16 lanes to a row 1.27, everything in float64 and walking down from the
-// top 4.6); 300 x 1500 ragged rows of 17 float16 logits with top-k 24 us (37).
+// 4096 x 1000 rows of 67 float32 logits with top-p 0.79 ms (16 lanes to a row 1.27, everything in float64 and walking down from the
+// top 4.6); 300 x 1500 ragged rows of 17 float16 logits with top-k 22 us (37).
 template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sample_short(SampleArgs a)
 {
     constexpr int RPG = 256 / G;
     const float NINF = -__builtin_inff();
     const int l = threadIdx.x % G, C = a.s.C;
     const int first = l * E, at = min(first, C - E);
-    const bool on = first < C;
+    const int skip = first < C ? first - at : E; // the elements of a chunk moved back that are its neighbour's; all of one behind the row
     const bool each = a.p.temperature_B || a.p.top_p_B || a.p.min_p_B || a.p.top_k_B;
     Draw d = draw_of(a, 0);
     for (uint32_t r = blockIdx.x * RPG + threadIdx.x / G; r < a.s.rows; r += gridDim.x * RPG) {
@@ -302,7 +303,7 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
             load_n<T, E>(row_in<T>(a.z, b, t) + at, z);
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                z[j] = (on && at + j >= first) ? clean(z[j]) : NINF;
+                z[j] = j >= skip ? clean(z[j]) : NINF;
                 m = fmaxf(m, z[j]);
             }
             m = group_all<G, OpMax>(m);
@@ -411,9 +412,9 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
 //   ranges that still hold too many (thousands of equal or extreme logits): the border is searched bit by bit, a sweep each.
 // The draw itself adds the kept masses of blocks of 64 vectors in index order.
 // Bound: the float64 exponentials of the histogram and of the draw where k does not bound the prefix, latency for few rows.  One
-// workgroup per CU (with two, 64 registers a thread, the float64 polynomial spills: 604 us instead of 235).
-// 512 rows of 131072 bfloat16 logits with parameters of their own 235 us (searching every border bit by bit: 2878), 8 rows of
-// 32000 float32 ones 49 us (472).
+// workgroup per CU (with two, 64 registers a thread, the float64 polynomial spills: 604 us instead of 235 at the time).
+// 512 rows of 131072 bfloat16 logits with parameters of their own 0.19 ms (searching every border bit by bit: 2.9), all with
+// k = 50 62 us, all with p = 0.9 0.3 ms; 8 rows of 32000 float32 logits 43 us (472).
 constexpr int SAMPLE_MAX_C = 1 << 19, SAMPLE_BLOCKS = SAMPLE_MAX_C / (64 * 4);
 constexpr int SAMPLE_LIST = 2048, SAMPLE_LIST_K = 224, SAMPLE_BINS = 2048;
 
@@ -434,7 +435,7 @@ template <typename T> struct LongRow {
     {
         const int n = C / VEC * VEC;
         int i = threadIdx.x * VEC;
-        for (; i + (U - 1) * 1024 * VEC < n; i += U * 1024 * VEC) {
+        for (; U > 1 && i + (U - 1) * 1024 * VEC < n; i += U * 1024 * VEC) {
             float v[U][VEC];
 #pragma unroll
             for (int k = 0; k < U; ++k) load_n<T, VEC>(z + i + k * 1024 * VEC, v[k]);
@@ -553,11 +554,11 @@ template <typename T> struct LongSampler {
             __syncthreads();
             row.template sweep<1>([&](int, float z) {
                 const float v = place(z);
+                // 2^52 + w 2^shift: its low bits are the whole number (not behind the branch: the vector's exponentials run side by side)
+                const double x = __builtin_fma(weight(z, m, inv_t), up, 4503599627370496.0);
                 if (z > -__builtin_inff() && v >= base && v < base + width) {
                     const int b = (int)((v - base) * fine);
                     atomicAdd(&sh.count[b], 1u);
-                    // 2^52 + w 2^shift: its low bits are the whole number
-                    const double x = __builtin_fma(weight(z, m, inv_t), up, 4503599627370496.0);
                     atomicAdd(&sh.bin[b], (unsigned long long)__double_as_longlong(x) & 0xfffffffffffffull);
                 }
             });
@@ -762,7 +763,7 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
                 continue;
             }
         }
-        uint32_t kt = 0; // kept: key > kt, and of the classes at kt the first `ties`
+        float zt = NINF; // kept: z > zt, and of the classes at zt the first `ties`
         int ties = a.s.C, all_ties = 0;
         double S = -1.0;
         if (d.k < a.s.C) {
@@ -771,14 +772,14 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
             n = block_all<W16, OpAdd>(n, sh.i, ti);
             if (d.k < n) {
                 own.locate(d.k, 0.0, 0.0);
-                kt = sh.kt; ties = sh.ties; all_ties = sh.all_ties; S = sh.S;
+                zt = value_of(sh.kt); ties = sh.ties; all_ties = sh.all_ties; S = sh.S;
             }
         }
         if (d.p < 1.0) {
             own.locate(0, d.p, S);
-            kt = sh.kt; ties = sh.ties; all_ties = sh.all_ties;
+            zt = value_of(sh.kt); ties = sh.ties; all_ties = sh.all_ties;
         }
-        // of classes at kt those in front of every block of BLOCK classes, where not all of them are kept
+        // of classes at zt those in front of every block of BLOCK classes, where not all of them are kept
         const int nb = (a.s.C + Row::BLOCK - 1) / Row::BLOCK;
         const bool cut = ties < all_ties;
         __syncthreads();
@@ -788,7 +789,7 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
                 int c = 0;
                 row.block(k, z);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) c += key_of(z[j]) == kt ? 1 : 0;
+                for (int j = 0; j < VEC; ++j) c += z[j] == zt ? 1 : 0;
                 c = group_all<64, OpAdd>(c);
                 if (lane == 0) sh.tied[k] = c;
             }
@@ -805,23 +806,28 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
             __syncthreads();
         }
         // the kept mass of every block, in index order
-        auto kept = [&](int k, float (&z)[VEC], double (&w)[VEC]) {
-            row.block(k, z);
+        auto kept = [&](int k, const float (&z)[VEC], double (&w)[VEC]) {
             int before = 0;
             if (cut) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) before += key_of(z[j]) == kt ? 1 : 0;
+                for (int j = 0; j < VEC; ++j) before += z[j] == zt ? 1 : 0;
                 before = sh.tied[k] + group_scan<64>(before, lane) - before;
             }
             double L = 0.0;
+            bool some = false;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { some |= z[j] >= zt; w[j] = 0.0; }
+            if (!__any(some)) return L;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const uint32_t key = key_of(z[j]);
-                bool keep = key >= kt;
-                if (cut && key == kt) { keep = before < ties; ++before; }
-                w[j] = 0.0;
-                if (keep) w[j] = weight(z[j], m, d.inv_t);
-                if (!(w[j] >= d.q)) w[j] = 0.0;
+                bool keep = z[j] >= zt;
+                if (cut) {
+                    const bool tie = z[j] == zt;
+                    keep &= !tie | (before < ties);
+                    before += tie ? 1 : 0;
+                }
+                const double x = weight(z[j], m, d.inv_t);
+                w[j] = (keep & (x >= d.q)) ? x : 0.0;
                 L += w[j];
             }
             return L;
@@ -829,6 +835,7 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
         for (int k = wave; k < nb; k += W16) {
             float z[VEC];
             double w[VEC];
+            row.block(k, z);
             const double L = group_all<64, OpAdd>(kept(k, z, w));
             if (lane == 0) sh.mass[k] = L;
         }
@@ -857,6 +864,7 @@ template <typename T> __global__ __launch_bounds__(1024, 4) void k_sample_long(S
             if (!any) { pick = last; before = last_before; }
             float z[VEC];
             double w[VEC];
+            row.block(pick, z);
             const double L = kept(pick, z, w);
             const double incl = group_scan<64>(L, lane) + before;
             const unsigned long long past = any ? __ballot(incl > target && L > 0.0) : 0ull, some = __ballot(L > 0.0);
