@@ -591,3 +591,68 @@ def test_sample_labels_of_long_rows(prm, dtype, gpu_device):
         z[:, 1, 50:] = -math.inf
         return z
     run_sample(1, 2, 9001, dtype, 102, prep=lumps, **prm)
+
+
+@pytest.mark.parametrize("rows,C,dtype", [(9001, 600, torch.float32), (2100, 5000, torch.float16), (1100, 5000, torch.float32), (700, 33000, torch.bfloat16),
+                                          (530, 70001, torch.bfloat16), (3, 140001, torch.bfloat16), (3, 70003, torch.float32)], ids=str)
+def test_label_loss_workgroups_take_several_rows(rows, C, dtype, gpu_device):
+    """more rows than workgroups, some of which do not count, so that rows are fetched ahead of their turn or not at all"""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    z = torch.randn(1, rows, C, generator=g, device="cuda").to(dtype)
+    labels = torch.randint(0, C, (1, rows), generator=g, device="cuda")
+    labels[torch.rand(1, rows, generator=g, device="cuda") < 0.3] = -1
+    weights = torch.rand(1, rows, generator=g, device="cuda")
+    weights[0, ::7] = 0.0
+    z[0, 5 if rows > 5 else 1] = float("nan")  # in a row that does not count
+    labels[0, 5 if rows > 5 else 1] = -1
+    n = rows - rows // 9
+    loss, grad = bfa.label_loss_and_grad(z, labels, weights=weights, lengths=[n], reduction="sum")
+    counts = (labels[0] >= 0) & (weights[0] > 0) & (torch.arange(rows, device="cuda") < n)
+    total = 0.0
+    for i in range(0, rows, 128):
+        s = slice(i, min(rows, i + 128))
+        zd = torch.where(counts[s, None], z[0, s].double(), 0.0)
+        lp, w = torch.log_softmax(zd, -1), torch.where(counts[s], weights[0, s].double(), 0.0)
+        at = labels[0, s].clamp(min=0)
+        total -= float((lp.gather(-1, at[:, None])[:, 0] * w).sum())
+        want = lp.exp()
+        want[torch.arange(want.shape[0], device="cuda"), at] -= 1.0
+        want *= w[:, None]
+        # a step of the type, and the exponent's roundings (|z| <= 6: at most 12 + 4 of them)
+        tol = half_step(dtype) * want.abs() + 32 * E * w[:, None] * (lp.exp() + (want < 0)) + 1e-30
+        if dtype == torch.float16:
+            tol = tol + 2.0 ** -25
+        assert bool(((grad[0, s].double() - want).abs() <= tol).all()), i
+    assert abs(float(loss) - total) <= 32 * E * abs(total) + E * rows
+
+
+def test_sample_labels_of_more_rows_than_workgroups(gpu_device):
+    g = torch.Generator(device="cuda").manual_seed(7)
+    for rows, C, cut in ((1500, 520, 1000), (600001, 5, 300000), (40000, 400, 30000)):
+        z, u = torch.randn(rows, C, generator=g, device="cuda"), torch.rand(rows, generator=g, device="cuda")
+        for prm in (dict(top_p=0.8), dict(top_k=3, temperature=0.7)):
+            got = bfa.sample_labels(z, u, **prm)
+            parts = [bfa.sample_labels(z[s], u[s], **prm) for s in (slice(0, cut), slice(cut, rows))]
+            assert torch.equal(got[0], torch.cat([p[0] for p in parts])) and torch.equal(got[1], torch.cat([p[1] for p in parts]))
+
+
+@pytest.mark.parametrize("C", [17, 67, 200, 500])
+def test_sample_labels_near_the_borders(C, gpu_device):
+    """numbers within a few steps of float32 of the borders between classes, and prefixes that end within them: the label is the
+    one float64 gives"""
+    z, zd = rows_of(1, 1, C, torch.float32, 111)
+    for top_p in (1.0, 0.9):
+        w = torch.exp(zd[0, 0] - zd.max())
+        order = torch.argsort(-w, stable=True)
+        front = torch.cumsum(w[order], 0) - w[order]
+        kept = torch.zeros(C, dtype=torch.bool)
+        kept[order[(front < float(torch.tensor(top_p)) * w.sum()) | (top_p == 1.0)]] = True
+        wk = torch.where(kept, w, 0.0)
+        borders = (torch.cumsum(wk, 0) / wk.sum()).float()
+        u = torch.cat([(borders.double() * (1 + k * 2.0 ** -24)).float() for k in (-40, -3, -1, 0, 1, 3, 40)]).clamp(0, 1 - 2.0 ** -24)
+        got = bfa.sample_labels(z.expand(1, len(u), C), u[None].cuda(), top_p=top_p)[0].cpu()[0]
+        run = torch.cumsum(wk, 0)
+        goal = u.double() * wk.sum()
+        want = (run[None] <= goal[:, None]).sum(1)
+        clear = ((run[None] - goal[:, None]).abs() > 1e-12 * C).all(1)  # (closer than the order of a float64 sum tells apart)
+        assert bool(clear.any()) and torch.equal(got[clear], want.int()[clear])
