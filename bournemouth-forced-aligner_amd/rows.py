@@ -62,6 +62,8 @@ def _rows(x, B, T):
 def _lengths(lengths, B, dev, what):
     if lengths is None:
         return None
+    if isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int32 and lengths.device == dev and lengths.shape == (B,):
+        return lengths.contiguous()
     n = len(lengths) if not isinstance(lengths, torch.Tensor) else lengths.numel()
     if n != B or (isinstance(lengths, torch.Tensor) and lengths.dim() != 1):
         raise ValueError(f"{what}: lengths must have one entry per utterance ({B})")
@@ -78,17 +80,29 @@ def _per_row(t, shape, dtype, dev, what, name):
         raise ValueError(f"{what}: {name} is on {t.device}, the rows on {dev}")
     if dtype == torch.int32 and (t.is_floating_point() or t.is_complex()):
         raise TypeError(f"{what}: {name} must be whole numbers")
-    return t.to(device=dev, dtype=dtype).contiguous()
+    if t.dtype != dtype or t.device != dev:
+        t = t.to(device=dev, dtype=dtype)
+    return t.contiguous()
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without the object around it, where this torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(dev):
     # (the C entries work on their handle's device, whatever the current one is)
-    L = _lib.lib()
-    return L, _lib.handle(dev.index), torch.cuda.current_stream(dev).cuda_stream
+    return _lib.lib(), _lib.handle(dev.index), _raw_stream(dev.index)
+
+
+def _backward_of(fn):
+    """fn(ctx, *gradients) as a backward pass that cannot be differentiated again; what that takes is spent only when a graph of the
+    gradients is built"""
+    once = torch.autograd.function.once_differentiable(fn)
+    return staticmethod(lambda ctx, *grads: (once if torch.is_grad_enabled() else fn)(ctx, *grads))
 
 
 # ---- layer normalisation ---------------------------------------------------------------------------------------------------
@@ -118,12 +132,12 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, lengths=None, statis
         raise ValueError("layer_norm: eps must not be negative")
     dev, C = x.device, x.shape[-1]
     lens = _lengths(lengths, B, dev, "layer_norm")
-    weight = None if weight is None else weight.detach().contiguous()
-    bias = None if bias is None else bias.detach().contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev) if statistics else None
     rstd = torch.empty_like(mean) if statistics else None
-    keep, rx = _rows(x.detach(), B, T)
+    keep, rx = _rows(x, B, T)
     ry = _lib.BfaRows(y.data_ptr(), rx.dtype, T * C, C)
     L, h, stream = _call(dev)
     rc = L.bfa_layer_norm(h, ctypes.byref(rx), B, T, C, _ptr(lens), _ptr(weight), _ptr(bias), wt, eps, ctypes.byref(ry),
@@ -148,15 +162,18 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, lengths=None, param_dt
     pdt = weight.dtype if weight is not None else (param_dtype or torch.float32)
     if pdt not in _DTYPES:
         raise TypeError("layer_norm_backward: param_dtype must be float32, float16 or bfloat16")
-    lens = _lengths(lengths, B, dev, "layer_norm_backward")
-    weight = None if weight is None else weight.detach().contiguous()
-    mean, rstd = mean.contiguous(), rstd.contiguous()
+    return _norm_backward(grad, x, mean.contiguous(), rstd.contiguous(), weight, _lengths(lengths, B, dev, "layer_norm_backward"), pdt, need, B, T)
+
+
+def _norm_backward(grad, x, mean, rstd, weight, lens, pdt, need, B, T):
+    dev, C = x.device, x.shape[-1]
+    weight = None if weight is None else weight.contiguous()
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
     make = torch.zeros if B * T == 0 else torch.empty
     dw = make(C, dtype=pdt, device=dev) if need[1] else None
     db = make(C, dtype=pdt, device=dev) if need[2] else None
-    kx, rx = _rows(x.detach(), B, T)
-    kg, rg = _rows(grad.detach(), B, T)
+    kx, rx = _rows(x, B, T)
+    kg, rg = _rows(grad, B, T)
     rdx = _lib.BfaRows(dx.data_ptr(), rx.dtype, T * C, C) if dx is not None else None
     L, h, stream = _call(dev)
     nbytes = L.bfa_layer_norm_workspace_bytes(B, T, C) if need[1] or need[2] else 0
@@ -176,19 +193,19 @@ class _LayerNorm(torch.autograd.Function):
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward_of
     def backward(ctx, grad):
-        x, weight, mean, rstd, lengths = ctx.saved_tensors
-        need = ctx.needs_input_grad[:3]
-        return (*layer_norm_backward(grad, x, mean, rstd, weight, lengths, ctx.bias_dtype, need), None, None)
+        x, weight, mean, rstd, lens = ctx.saved_tensors
+        B, T = _shape_of(x, lens, "layer_norm")
+        pdt = weight.dtype if weight is not None else (ctx.bias_dtype or torch.float32)
+        return (*_norm_backward(grad, x, mean, rstd, weight, lens, pdt, ctx.needs_input_grad[:3], B, T), None, None)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, lengths=None):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, differentiable in x, weight and bias.  weight and bias
     [C] have one type, the rows' or another of the three; mean, variance and all sums are float32."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
-        _check_rows(x, "layer_norm")
+    _check_rows(x, "layer_norm")
+    if torch.is_grad_enabled() and (x.requires_grad or getattr(weight, "requires_grad", False) or getattr(bias, "requires_grad", False)):
         B, _ = _shape_of(x, lengths, "layer_norm")
         return _LayerNorm.apply(x, weight, bias, eps, _lengths(lengths, B, x.device, "layer_norm"))
     return layer_norm_forward(x, weight, bias, eps, lengths, statistics=False)[0]
@@ -213,7 +230,7 @@ def _loss_call(logits, labels, weights, lens, reduction, want_loss, want_grad, s
     make = torch.zeros if C == 0 else torch.empty
     loss = make(logits.shape[:-1] if red == _lib.LOSS_NONE else (), dtype=torch.float32, device=dev) if want_loss else None
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-    keep, rz = _rows(logits.detach(), B, T)
+    keep, rz = _rows(logits, B, T)
     rg = _lib.BfaRows(grad.data_ptr(), rz.dtype, T * C, C) if want_grad else None
     L, h, stream = _call(dev)
     nbytes = L.bfa_label_loss_workspace_bytes(B, T, C) if red != _lib.LOSS_NONE else 0
@@ -231,8 +248,7 @@ class _LabelLoss(torch.autograd.Function):
         ctx.reduction = reduction
         return _loss_call(logits, labels, weights, lens, reduction, True, False)[0]
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward_of
     def backward(ctx, upstream):
         logits, labels, weights, lens = ctx.saved_tensors
         upstream = upstream.to(torch.float32).contiguous()
