@@ -792,6 +792,7 @@ static const char *bad_shape(int B, int T, int C, bool *empty)
 {
     if (B < 0 || T < 0 || C < 0) return "negative shape";
     if ((int64_t)B * T >= (1ll << 31)) return "B * T must be below 2^31";
+    if (C > (1 << 30)) return "C must be at most 2^30"; // (the kernels' 32-bit indexes run past the row by a stride)
     *empty = B == 0 || T == 0 || C == 0;
     return nullptr;
 }

@@ -44,8 +44,8 @@ def _shape_of(x, lengths, what):
         B, T = lead.numel(), 1
     if B * T >= 1 << 31:
         raise ValueError(f"{what}: at most 2^31 - 1 rows")
-    if x.shape[-1] >= 1 << 31:
-        raise ValueError(f"{what}: rows of at most 2^31 - 1 elements")
+    if x.shape[-1] > 1 << 30:
+        raise ValueError(f"{what}: rows of at most 2^30 elements")
     return B, T
 
 

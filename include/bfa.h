@@ -370,7 +370,7 @@ int bfa_index_records(bfa_handle h, const int32_t *records, int world, int64_t w
  * normalisation, the loss of the logits against the labels an alignment gives (out_frame_phoneme), labels drawn from the logits
  * -- with the gradients a model is trained by.  Rows are float32, float16 or bfloat16 (every bfa_rows of a call has the same
  * type); element (b,t,c) is data[b*strideB + t*strideT + c], strides in elements, any alignment that the type allows.  T_len
- * [B] int32 or NULL: rows t >= T_len[b] are not read, and written as said below.  B * T < 2^31; a call with B, T or C == 0 does
+ * [B] int32 or NULL: rows t >= T_len[b] are not read, and written as said below.  B * T < 2^31, C <= 2^30; a call with B, T or C == 0 does
  * nothing (a loss that is one number is then 0).  Sums and statistics are float32 or wider, in a fixed order: the
  * same call gives the same bits.  These calls keep nothing in the handle but the error text, may be captured into a graph, and
  * use `workspace` only until the stream has passed them -- calls on different streams need different ones.  Outputs do not overlap

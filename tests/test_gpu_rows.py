@@ -656,3 +656,18 @@ def test_sample_labels_near_the_borders(C, gpu_device):
         want = (run[None] <= goal[:, None]).sum(1)
         clear = ((run[None] - goal[:, None]).abs() > 1e-12 * C).all(1)  # (closer than the order of a float64 sum tells apart)
         assert bool(clear.any()) and torch.equal(got[clear], want.int()[clear])
+
+
+def test_rows_of_more_elements_than_indexes_reach_are_refused(gpu_device):
+    x = torch.zeros(1, 1, 1, device="cuda").expand(1, 1, (1 << 30) + 1)
+    for call in (lambda: bfa.layer_norm(x), lambda: bfa.label_loss(x, torch.zeros(1, 1, dtype=torch.int32, device="cuda")),
+                 lambda: bfa.sample_labels(x, torch.zeros(1, 1, device="cuda"))):
+        with pytest.raises(ValueError, match="2\\^30"):
+            call()
+
+
+@pytest.mark.parametrize("prm", [dict(), dict(top_k=50), dict(top_p=0.9), dict(top_k=100000, top_p=0.5)], ids=str)
+def test_sample_labels_of_the_longest_rows(prm, gpu_device):
+    C = 1 << 19
+    run_sample(1, 1, C, torch.float32, 121, **prm)
+    run_sample(1, 1, C, torch.bfloat16, 122, prep=lambda z: z.zero_(), **prm)
