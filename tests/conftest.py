@@ -13,20 +13,6 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
-# Not run, with the reason: a memory fault on the GPU is not sent there again before its cause is shown.
-NOT_RUN = {
-    "test_gpu_parity.py::test_soak_slice": "one of its randomized calls ended with an illegal address in the first run after the lane masks of K1 "
-                                           "went to vector stores; the cause is not shown yet (all other tests pass)",
-}
-
-
-def pytest_collection_modifyitems(config, items):
-    for item in items:
-        for name, reason in NOT_RUN.items():
-            if item.nodeid.endswith(name):
-                item.add_marker(pytest.mark.skip(reason=reason))
-
-
 @pytest.fixture(scope="session")
 def ora():
     from oracle import oracle
