@@ -282,7 +282,7 @@ def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
 
     `uniform`: one number in [0, 1) per row; the label is the lowest class up to which, in the order of the classes, more than that share
     of the kept probability lies, so the same numbers give the same labels.  The parameters are numbers, or tensors [B] with
-    one per utterance (sequence); they are taken as float32.  temperature 0 takes the most probable class (of equals the lowest).
+    one per utterance (sequence), or one number in a tensor; they are taken as float32.  temperature 0 takes the most probable class (of equals the lowest).
     -inf masks a class and NaN counts as -inf; rows with nothing left, and rows behind `lengths`, give label -1 and logp 0."""
     _check_rows(logits, "sample_labels")
     B, T = _shape_of(logits, lengths, "sample_labels")
@@ -293,8 +293,8 @@ def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     keep = []
     for name, value, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                             ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(value, torch.Tensor) and value.dim() > 0:
-            value = _per_row(value, (B,), dt, dev, "sample_labels", name)
+        if isinstance(value, torch.Tensor) and (value.dim() > 0 or value.is_cuda):  # (one number on the device is not read here)
+            value = _per_row(value if value.dim() > 0 else value.expand(B), (B,), dt, dev, "sample_labels", name)
             keep.append(value)
             setattr(p, name + "_B", value.data_ptr())
             continue

@@ -1,0 +1,51 @@
+"""What the row operators hand to the library, without a GPU: host tensors that say they are on one, and a library that notes its calls."""
+import pytest
+import torch
+
+import bournemouth_forced_aligner_amd as bfa
+from bournemouth_forced_aligner_amd import _lib, rows
+
+
+class _Device(torch.Tensor):
+    """a host tensor that says it is on the GPU and whose numbers cannot be read by the host"""
+    is_cuda = property(lambda self: True)
+
+    def _read(self, *args):
+        raise AssertionError("read by the host")
+
+    __bool__ = __float__ = __int__ = __index__ = item = tolist = cpu = _read
+
+
+def _device(t):
+    return t.as_subclass(_Device)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """the C entries as {name: arguments of its last call}"""
+    seen = {}
+
+    class Library:
+        def __getattr__(self, name):
+            def entry(*args):
+                seen[name] = args
+                return 0
+            return entry
+
+    monkeypatch.setattr(rows, "_call", lambda dev: (Library(), None, 0))
+    return seen
+
+
+def _sample_params(calls):
+    return calls["bfa_sample_labels"][7]._obj
+
+
+@pytest.mark.parametrize("name,value", [("temperature", 0.5), ("top_p", 0.25), ("min_p", 0.125), ("top_k", 3)])
+def test_one_number_on_the_device_is_not_read_by_the_host(calls, name, value):
+    x = _device(torch.zeros(4, 3, 8))
+    bfa.sample_labels(x, torch.zeros(4, 3), **{name: _device(torch.tensor(value))})
+    p = _sample_params(calls)
+    assert getattr(p, name + "_B")  # an array of B numbers, not a number
+    bfa.sample_labels(x, torch.zeros(4, 3), **{name: torch.tensor(value)})  # (one on the host is a number like any other)
+    p = _sample_params(calls)
+    assert not getattr(p, name + "_B") and getattr(p, name) == value
