@@ -294,6 +294,8 @@ def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     for name, value, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                             ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if isinstance(value, torch.Tensor) and (value.dim() > 0 or value.is_cuda):  # (one number on the device is not read here)
+            if value.dtype == torch.int64 and dt == torch.int32:
+                value = value.clamp(0, 0x7fffffff)  # (as a number is: a value of 33 bits does not come out as its low 32)
             value = _per_row(value if value.dim() > 0 else value.expand(B), (B,), dt, dev, "sample_labels", name)
             keep.append(value)
             setattr(p, name + "_B", value.data_ptr())

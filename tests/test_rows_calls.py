@@ -49,3 +49,14 @@ def test_one_number_on_the_device_is_not_read_by_the_host(calls, name, value):
     bfa.sample_labels(x, torch.zeros(4, 3), **{name: torch.tensor(value)})  # (one on the host is a number like any other)
     p = _sample_params(calls)
     assert not getattr(p, name + "_B") and getattr(p, name) == value
+
+
+@pytest.mark.parametrize("k,want", [(2 ** 32 + 5, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (-2 ** 33 - 1, 0), (7, 7), (-1, 0)])
+def test_a_wide_top_k_is_as_much_as_fits(calls, monkeypatch, k, want):
+    given = []
+    kept = rows._per_row
+    monkeypatch.setattr(rows, "_per_row", lambda *args: given.append(kept(*args)) or given[-1])
+    bfa.sample_labels(_device(torch.zeros(2, 3, 8)), torch.zeros(2, 3), top_k=torch.tensor([k, 4]))
+    assert given[-1].dtype == torch.int32 and given[-1].tolist() == [want, 4]
+    bfa.sample_labels(_device(torch.zeros(2, 3, 8)), torch.zeros(2, 3), top_k=k)
+    assert _sample_params(calls).top_k == want
