@@ -256,9 +256,12 @@ class _LabelLoss(torch.autograd.Function):
 
 
 def label_loss(logits, labels, weights=None, lengths=None, reduction="mean"):
-    """Weighted cross entropy -weight * log softmax(logits)[label] of every row, float32, differentiable in the logits.  Rows with
-    a negative label (an alignment's -1) or weight 0 and rows behind `lengths` give 0; a label >= C gives NaN (labels are taken as int32).  reduction: 'none' (one per row),
-    'sum', or 'mean' (divided by the sum of the weights of the rows that count; 0 where that is 0)."""
+    """Weighted cross entropy -weight * log softmax(logits)[label] of every row, float32, differentiable in the logits (not in the
+    weights: those that require a gradient are refused).  Rows with a negative label (an alignment's -1) or weight 0 and rows behind
+    `lengths` give 0; a label >= C gives NaN (labels are taken as int32).  reduction: 'none' (one per row), 'sum', or 'mean' (divided
+    by the sum of the weights of the rows that count; 0 where that is 0)."""
+    if torch.is_grad_enabled() and getattr(weights, "requires_grad", False):
+        raise ValueError("label_loss: no gradient goes to the weights: pass weights.detach()")
     labels, weights, lens = _loss_args(logits, labels, weights, lengths, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _LabelLoss.apply(logits, labels, weights, lens, reduction)

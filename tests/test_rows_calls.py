@@ -60,3 +60,15 @@ def test_a_wide_top_k_is_as_much_as_fits(calls, monkeypatch, k, want):
     assert given[-1].dtype == torch.int32 and given[-1].tolist() == [want, 4]
     bfa.sample_labels(_device(torch.zeros(2, 3, 8)), torch.zeros(2, 3), top_k=k)
     assert _sample_params(calls).top_k == want
+
+
+def test_weights_that_require_a_gradient_are_refused(calls):
+    x, labels = _device(torch.zeros(2, 3, 8)), torch.zeros(2, 3, dtype=torch.int32)
+    w = torch.ones(2, 3, requires_grad=True)
+    for rows_in in (x, _device(torch.zeros(2, 3, 8)).requires_grad_()):
+        with pytest.raises(ValueError, match="no gradient goes to the weights"):
+            bfa.label_loss(rows_in, labels, weights=w)
+    bfa.label_loss(x, labels, weights=w.detach())
+    with torch.no_grad():
+        bfa.label_loss(x, labels, weights=w)
+    bfa.label_loss_and_grad(x, labels, weights=w)  # (builds no graph: the gradient it returns is the logits')
