@@ -14,6 +14,7 @@ A backward pass may be captured into a graph like the forward pass.  PyTorch end
 import ctypes
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from .forced_alignment import HostLens, _as_i32
@@ -98,6 +99,18 @@ def _call(dev):
     return _lib.lib(), _lib.handle(dev.index), _raw_stream(dev.index)
 
 
+def _tangent(t):
+    return _forward_ad.unpack_dual(t).tangent if _forward_ad._current_level >= 0 and isinstance(t, torch.Tensor) else None
+
+
+def _wants_graph(*tensors):
+    """whether a call has to go through its autograd function: an input requires a gradient, or forward-mode differentiation is on
+    (the functions have no rule for it, and torch says so where an input has a tangent)"""
+    if _forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors)
+
+
 def _backward_of(fn):
     """fn(ctx, *gradients) as a backward pass that cannot be differentiated again; what that takes is spent only when a graph of the
     gradients is built"""
@@ -123,7 +136,7 @@ def _norm_params(x, weight, bias):
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, lengths=None, statistics=True):
-    """(y, mean, rstd): y as `layer_norm` gives it (without a gradient), the rows' statistics float32 of the leading shape (None,
+    """(y, mean, rstd): y as `layer_norm` gives it (without a gradient of either mode), the rows' statistics float32 of the leading shape (None,
     None without `statistics`) as `layer_norm_backward` takes them."""
     _check_rows(x, "layer_norm")
     B, T = _shape_of(x, lengths, "layer_norm")
@@ -205,7 +218,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, lengths=None):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, differentiable in x, weight and bias.  weight and bias
     [C] have one type, the rows' or another of the three; mean, variance and all sums are float32."""
     _check_rows(x, "layer_norm")
-    if torch.is_grad_enabled() and (x.requires_grad or getattr(weight, "requires_grad", False) or getattr(bias, "requires_grad", False)):
+    if _wants_graph(x, weight, bias):
         B, _ = _shape_of(x, lengths, "layer_norm")
         return _LayerNorm.apply(x, weight, bias, eps, _lengths(lengths, B, x.device, "layer_norm"))
     return layer_norm_forward(x, weight, bias, eps, lengths, statistics=False)[0]
@@ -260,10 +273,10 @@ def label_loss(logits, labels, weights=None, lengths=None, reduction="mean"):
     weights: those that require a gradient are refused).  Rows with a negative label (an alignment's -1) or weight 0 and rows behind
     `lengths` give 0; a label >= C gives NaN (labels are taken as int32).  reduction: 'none' (one per row), 'sum', or 'mean' (divided
     by the sum of the weights of the rows that count; 0 where that is 0)."""
-    if torch.is_grad_enabled() and getattr(weights, "requires_grad", False):
+    if (torch.is_grad_enabled() and getattr(weights, "requires_grad", False)) or _tangent(weights) is not None:
         raise ValueError("label_loss: no gradient goes to the weights: pass weights.detach()")
     labels, weights, lens = _loss_args(logits, labels, weights, lengths, reduction)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _wants_graph(logits):
         return _LabelLoss.apply(logits, labels, weights, lens, reduction)
     return _loss_call(logits, labels, weights, lens, reduction, True, False)[0]
 
@@ -281,7 +294,7 @@ def label_loss_and_grad(logits, labels, weights=None, lengths=None, reduction="m
 def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, lengths=None):
     """(labels int32, logp float32) of the rows' leading shape: one class per row from softmax(logits / temperature), kept to the
     `top_k` most probable classes (0: all), of those to the fewest that hold `top_p` of their probability, and to classes with at least
-    `min_p` of the greatest probability; logp is the logarithm of the drawn class's probability among the kept ones.
+    `min_p` of the greatest probability; logp is the logarithm of the drawn class's probability among the kept ones (without a gradient).
 
     `uniform`: one number in [0, 1) per row; the label is the lowest class up to which, in the order of the classes, more than that share
     of the kept probability lies, so the same numbers give the same labels.  The parameters are numbers, or tensors [B] with

@@ -1,6 +1,7 @@
 """What the row operators hand to the library, without a GPU: host tensors that say they are on one, and a library that notes its calls."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import bournemouth_forced_aligner_amd as bfa
 from bournemouth_forced_aligner_amd import _lib, rows
@@ -72,3 +73,18 @@ def test_weights_that_require_a_gradient_are_refused(calls):
     with torch.no_grad():
         bfa.label_loss(x, labels, weights=w)
     bfa.label_loss_and_grad(x, labels, weights=w)  # (builds no graph: the gradient it returns is the logits')
+
+
+def test_tangents_are_refused_not_dropped(calls):
+    x, w, labels = torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(2, 3, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(_device(x), _device(torch.ones_like(x)))
+        dual_w = forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: bfa.layer_norm(dual), lambda: bfa.layer_norm(_device(x), dual_w), lambda: bfa.label_loss(dual, labels)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call()
+        with pytest.raises(ValueError, match="no gradient goes to the weights"):
+            bfa.label_loss(_device(x), labels, weights=forward_ad.make_dual(torch.ones(2, 3), torch.ones(2, 3)))
+        bfa.layer_norm(_device(x), w)  # (without a tangent: as ever)
+        bfa.label_loss(_device(x), labels)
+    assert {"bfa_layer_norm", "bfa_label_loss"} <= set(calls)
