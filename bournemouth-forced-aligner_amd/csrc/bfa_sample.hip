@@ -46,12 +46,12 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs &a, uint32_t b)
 }
 
 // y r + c with the constant in a pair of scalar registers (left to itself the compiler moves every constant of a polynomial into
-// vector registers first, an instruction each)
+// vector registers first, an instruction each).  The product itself is the compiler's: in inline asm it would not be kept apart from a
+// v_readlane that has just brought a spilled constant back.
 __device__ __forceinline__ double fma_c(double y, double r, double c)
 {
-    double o;
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(o) : "v"(y), "v"(r), "s"(c));
-    return o;
+    asm("" : "+s"(c));
+    return __builtin_fma(y, r, c);
 }
 // e^x, x <= 0, to about one unit in the last place: x = n ln 2 + r, |r| <= ln 2 / 2, the Taylor polynomial of degree 12
 // (remainder 0.3466^13 / 13! < 2^-52); -inf and NaN give 0.  The sum with 1.5 2^52 rounds to a whole number and holds it in its low

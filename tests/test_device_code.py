@@ -88,3 +88,16 @@ def test_no_spill_under_a_narrow_lane_mask(tmp_path):
     with ThreadPoolExecutor(4) as pool:
         found = [x for part in pool.map(scan, enumerate(images)) for x in part]
     assert not found, found
+
+
+def test_no_vector_instruction_in_inline_asm_reads_a_scalar_register():
+    """The compiler keeps its own vector instructions apart from a v_readlane that has just brought a spilled scalar register back; it
+    does not look into inline asm."""
+    src = os.path.join(ROOT, "bournemouth-forced-aligner_amd", "csrc")
+    for name in sorted(os.listdir(src)):
+        if not name.endswith((".hip", ".inc", ".hpp", ".cpp")):
+            continue
+        for statement in re.findall(r"\basm\b(?:\s+volatile)?\s*\((.*?)\);", open(os.path.join(src, name)).read(), flags=re.S):
+            code, _, operands = statement.partition(":")
+            if re.search(r'"\s*v_|\\tv_', code):
+                assert not re.search(r'"\+?s"\s*\(', operands), f"{name}: {statement[:200]}"
