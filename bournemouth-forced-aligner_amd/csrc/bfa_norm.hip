@@ -6,16 +6,17 @@
 // Rows behind T_len[b] are not read: y = 0, mean = rstd = 0, dx = 0, and nothing of them goes into dw / db.
 //
 // Bound: HBM.  A row is read once and stays in the registers of the TPR threads that share it (at most 16 elements each), so
-// the variance is the two-pass one (deviations from the mean, float32) at no extra traffic.  The last 16-byte vector of a row is
+// the variance is the two-pass one (deviations from the mean, float32) at no extra traffic, and the mean's own rounding is taken
+// from the deviations again (norm_stat).  The last 16-byte vector of a row is
 // moved back to end with the row where C is not a multiple of it -- wide loads and stores for every C and every alignment; the
 // elements it shares with its neighbour are counted once (`own`) and stored twice with the same value.
 // Workgroups stride over the rows: the weights are loaded once per workgroup, and in the backward pass a thread keeps the sums
 // of its own columns in registers.  Per workgroup one partial sum per column goes to the workspace, and k_norm_cols adds those
 // in a fixed order: no atomics, the same bits every time.
 //
-// Measured: 32768 rows of 4096 bfloat16 channels 102 us forward (5.3 TB/s), 168 us backward (4.8 TB/s) + 6.6 for the column sums; 16
-// ragged utterances of up to 1870 x 768 float32 25 + 36 + 5 us; 12000 ragged rows of 1001 float16 channels, every row at another
-// alignment, 11 + 15 + 6 us (35 + 21 with the weights loaded one by one).
+// Measured: 32768 rows of 4096 bfloat16 channels 104 us forward (5.2 TB/s; 100 without the correction of the mean), 168 us backward
+// (4.8 TB/s) + 6.5 for the column sums; 16 ragged utterances of up to 1870 x 768 float32 24 + 35 + 5 us; 12000 ragged rows of 1001
+// float16 channels, every row at another alignment, 11 + 15 + 6 us (35 + 21 with the weights loaded one by one).
 #include <algorithm>
 
 #include "bfa_rows.hpp"
@@ -43,12 +44,37 @@ template <int TPR> __device__ __forceinline__ float norm_sum(float v, float *sm,
     if constexpr (TPR <= 64) return group_all<TPR, OpAdd>(v);
     else return block_all<TPR / 64, OpAdd>(v, sm, turn);
 }
+// the sums of two numbers behind one barrier (sm: 4 * W entries)
+template <int TPR> __device__ __forceinline__ void norm_sum2(float &a, float &b, float *sm, int &turn)
+{
+    constexpr int W = TPR / 64;
+    a = group_all<(TPR < 64 ? TPR : 64), OpAdd>(a);
+    b = group_all<(TPR < 64 ? TPR : 64), OpAdd>(b);
+    if constexpr (W > 1) {
+        float *s = sm + (turn ? 2 * W : 0);
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = a; s[W + (threadIdx.x >> 6)] = b; }
+        __syncthreads();
+        a = s[0];
+        b = s[W];
+#pragma unroll
+        for (int k = 1; k < W; ++k) { a += s[k]; b += s[W + k]; }
+    }
+}
+// Mean and rstd of a row from its deviations from a first mean m (their sum and the sum of their squares).  The deviations of a row whose
+// mean is large against its spread are exact, the mean itself is rounded: what it lacks, `shift`, is the deviations' mean.
+struct NormStat { float shift, rstd; };
+__device__ __forceinline__ NormStat norm_stat(float sum, float squares, float inv_c, float eps)
+{
+    const float shift = sum * inv_c, var = squares * inv_c - shift * shift;
+    return {shift, 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps)}; // (NaN stays)
+}
 
 template <typename T, int VEC, int TPR, int NV>
 __global__ __launch_bounds__(NormGeo<TPR>::WG) void k_norm(NormArgs a)
 {
     using Geo = NormGeo<TPR>;
-    __shared__ float sm[2 * Geo::W];
+    __shared__ float sm[4 * Geo::W];
     const int l = threadIdx.x % TPR, C = a.s.C;
     const float inv_c = 1.0f / (float)C;
     int turn = 0;
@@ -76,20 +102,25 @@ __global__ __launch_bounds__(NormGeo<TPR>::WG) void k_norm(NormArgs a)
             for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s += own(v, j) ? x[v][j] : 0.0f;
-            mean = norm_sum<TPR>(s, sm, turn) * inv_c;
+            mean = norm_sum<TPR>(s, sm, turn) / (float)C;
+            float q = 0.0f;
             s = 0.0f;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     x[v][j] -= mean;
-                    s = own(v, j) ? __builtin_fmaf(x[v][j], x[v][j], s) : s;
+                    s += own(v, j) ? x[v][j] : 0.0f;
+                    q = own(v, j) ? __builtin_fmaf(x[v][j], x[v][j], q) : q;
                 }
-            rstd = 1.0f / sqrtf(norm_sum<TPR>(s, sm, turn) * inv_c + a.eps);
+            norm_sum2<TPR>(s, q, sm, turn);
+            const NormStat st = norm_stat(s, q, inv_c, a.eps);
+            rstd = st.rstd;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) x[v][j] = __builtin_fmaf(x[v][j] * rstd, w[v][j], b[v][j]);
+                for (int j = 0; j < VEC; ++j) x[v][j] = __builtin_fmaf((x[v][j] - st.shift) * rstd, w[v][j], b[v][j]);
+            mean += st.shift;
         } else {
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -198,14 +229,14 @@ __global__ __launch_bounds__(NormGeo<TPR>::WG) void k_norm_bwd(NormArgs a)
 template <typename T> __global__ __launch_bounds__(1024) void k_norm_long(NormArgs a)
 {
     constexpr int VEC = 16 / sizeof(T);
-    __shared__ float sm[32];
+    __shared__ float sm[64];
     const int C = a.s.C, n = C / VEC * VEC;
     int turn = 0;
     for (uint32_t r = blockIdx.x; r < a.s.rows; r += gridDim.x) {
         uint32_t bb, t;
         a.s.split(r, bb, t);
         T *y = row_out<T>(a.y, bb, t);
-        float mean = 0.0f, rstd = 0.0f;
+        float mean = 0.0f, shift = 0.0f, rstd = 0.0f;
         const bool held = a.s.held(bb, t);
         const T *px = row_in<T>(a.x, bb, t);
         if (held) {
@@ -216,21 +247,26 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_long(NormAr
                 for (int j = 0; j < VEC; ++j) s += x[j];
             }
             if (n + (int)threadIdx.x < C) s += (float)px[n + threadIdx.x];
-            mean = block_all<16, OpAdd>(s, sm, turn) / (float)C;
+            mean = norm_sum<1024>(s, sm, turn) / (float)C;
+            float q = 0.0f;
             s = 0.0f;
             for (int i = threadIdx.x * VEC; i < n; i += 1024 * VEC) {
                 load_n<T, VEC>(px + i, x);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) { const float d = x[j] - mean; s = __builtin_fmaf(d, d, s); }
+                for (int j = 0; j < VEC; ++j) { const float d = x[j] - mean; s += d; q = __builtin_fmaf(d, d, q); }
             }
-            if (n + (int)threadIdx.x < C) { const float d = (float)px[n + threadIdx.x] - mean; s = __builtin_fmaf(d, d, s); }
-            rstd = 1.0f / sqrtf(block_all<16, OpAdd>(s, sm, turn) / (float)C + a.eps);
+            if (n + (int)threadIdx.x < C) { const float d = (float)px[n + threadIdx.x] - mean; s += d; q = __builtin_fmaf(d, d, q); }
+            norm_sum2<1024>(s, q, sm, turn);
+            const NormStat st = norm_stat(s, q, 1.0f / (float)C, a.eps);
+            shift = st.shift;
+            rstd = st.rstd;
         }
         for (int i = threadIdx.x; i < C; i += 1024) {
-            const float v = held ? __builtin_fmaf(((float)px[i] - mean) * rstd, a.w ? load_w(a.w, a.wtype, i) : 1.0f,
+            const float v = held ? __builtin_fmaf((((float)px[i] - mean) - shift) * rstd, a.w ? load_w(a.w, a.wtype, i) : 1.0f,
                                                   a.b ? load_w(a.b, a.wtype, i) : 0.0f) : 0.0f;
             y[i] = (T)v;
         }
+        mean += shift;
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
