@@ -191,7 +191,11 @@ template <typename T> struct Packed {
     // what was unpacked before is not kept for later (the registers hold the row as stored, not as floats too)
     __device__ __forceinline__ void forget() { asm volatile("" : "+v"(u[0]), "+v"(u[1]), "+v"(u[2]), "+v"(u[3])); }
 };
-// e^x, x <= 0: 16-bit logits take the plain product (its error, |x| 2^-24 of a weight e^x, is far below their rounding)
+// e^x, x <= 0: 16-bit logits take the plain product, which is off by |x| 2^-24 of a weight e^x.  The gradient is rounded to 2^-9 or
+// 2^-12 behind it.  In log(sum) it is 2^-24 times the mean |x| under the softmax, at most ln C (7 2^-24 for 131072 normal logits): no more
+// than the sum's own additions and the rounding of the loss.  Losses of 131072 bfloat16 and 5003 float16 classes against float64, rms:
+// 8.2, 7.2 2^-24 (normal), 3.3 (one class in front), 17.6 (one class 8 to 11 in front of all others alike); by exp_neg 7.9, 7.4, 3.4, 16.5,
+// and 1.5 to 14 % slower.
 template <typename T> __device__ __forceinline__ float exp_row(float x)
 {
     if constexpr (sizeof(T) == 4) return exp_neg(x);
