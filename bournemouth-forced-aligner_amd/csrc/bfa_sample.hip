@@ -116,10 +116,16 @@ template <int G, typename V> __device__ __forceinline__ V group_scan(V x, int l)
 }
 
 // A row's draw in float32, by a group of G lanes of E consecutive classes each (z: -inf where a lane has none): false where a
-// border lies within the error of the sums, so that the decision is left to float64.
-//   w = 2^((z - m) log2(e) / T) carries three roundings of its exponent: |x| 3 2^-24 w <= 1.1 2^-24, and the exponential's 2^-23 w;
-//   a sum over the row adds at most 14 more to its terms.  So a sum is off by less than (1.25 C + 20 S) 2^-24, and a difference of a
-//   sum and p S or u W by less than three times that.
+// border lies within the error of the sums, so that the decision is left to float64.  In units of 2^-24, with A = log2 G steps over the lanes:
+//   a weight 2^((z - m) log2(e) / T) carries three roundings of its exponent, |x| 3 w <= 1.11, and the exponential's 2 w: 1.11 C + 2 S
+//   in any sum over the row;
+//   a prefix up to a value adds E + A times, then once for a number of equal weights and once for their product at each of `steps`
+//   values walked past, and twice at the last: 2 S + (E + A + 2 steps + 2) S;  p S: (E + A + 2 + 1) S;
+//   the mass up to a class adds E times in the lanes in front, A over them, once more and E times in its own lane: (2 E + A + 1) S;
+//   u W: (E + A + 1) S.
+// So a prefix and p S differ by at most 2.22 C + (2 E + 2 A + 2 steps + 9) S more or less than they seem to, the mass up to a class
+// and u W by 2.22 C + (3 E + 2 A + 6) S.  Only the label is certain in this way: logp is the float32 logarithm of W, off by
+// (1.11 C / W + E + A + 2) 2^-24 and by the roundings of the logarithm itself.
 template <int G, int E>
 __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, float m, const Draw &d, float u, int l, int &label, float &logp)
 {
@@ -130,7 +136,8 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
 #pragma unroll
     for (int j = 0; j < E; ++j) { w[j] = __builtin_amdgcn_exp2f((z[j] - m) * rate); S += w[j]; }
     S = group_all<G, OpAdd>(S);
-    const float tol = (1.25f * (float)C + 20.0f * S) * (3.0f / 16777216.0f);
+    constexpr float U = 1.0f / 16777216.0f, ADDS = 3 * E + (G == 4 ? 4 : G == 16 ? 8 : 12) + 10;
+    const float tol = (2.25f * (float)C + ADDS * S) * U; // (U, ADDS: covers either bound without `steps`)
     float zt = NINF; // kept: z > zt, and of the classes at zt the first `ties`
     int ties = C;
     bool cut = false, sure = true;
@@ -205,7 +212,7 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
             hi = below ? mid : hi;
             lo = below ? lo : mid;
         }
-        float v = next_from(hi);
+        float v = next_from(hi), walked = tol;
         sure = false;
         while (v > NINF) {
             const int c = count_at(v);
@@ -215,10 +222,11 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
                 zt = v;
                 ties = (int)r;
                 cut = ties < c;
-                sure = target - (M + (r - 1.0f) * wv) > tol && (M + r * wv) - target > tol;
+                sure = target - (M + (r - 1.0f) * wv) > walked && (M + r * wv) - target > walked;
                 break;
             }
             M += (float)c * wv;
+            walked += 2.0f * U * S;
             v = next_below(v);
         }
     }

@@ -294,7 +294,8 @@ def label_loss_and_grad(logits, labels, weights=None, lengths=None, reduction="m
 def sample_labels(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, lengths=None):
     """(labels int32, logp float32) of the rows' leading shape: one class per row from softmax(logits / temperature), kept to the
     `top_k` most probable classes (0: all), of those to the fewest that hold `top_p` of their probability, and to classes with at least
-    `min_p` of the greatest probability; logp is the logarithm of the drawn class's probability among the kept ones (without a gradient).
+    `min_p` of the greatest probability; logp is the logarithm of the drawn class's probability among the kept ones (without a
+    gradient; up to 512 classes from a float32 sum, good to about 2^-22).
 
     `uniform`: one number in [0, 1) per row; the label is the lowest class up to which, in the order of the classes, more than that share
     of the kept probability lies, so the same numbers give the same labels.  The parameters are numbers, or tensors [B] with

@@ -416,7 +416,10 @@ int bfa_label_loss(bfa_handle h, const bfa_rows *logits, int B, int T, int C, co
  * descending, index ascending): at most top_k of them (<= 0: all), the fewest whose probability within those reaches top_p (>= 1:
  * all), those with at least min_p of the greatest probability; the first class always stays.  With W the weight that is left,
  * out_label [B,T] int32 is the lowest index up to which, in index order, more than uniform[b,t] * W is reached (numbers outside [0,1)
- * count as the nearest inside, NaN as 0), out_logp [B,T] float32 (or NULL) the logarithm of its probability within W.
+ * count as the nearest inside, NaN as 0), out_logp [B,T] float32 (or NULL) the logarithm of its probability within W.  The label is the one of
+ * the exact weights unless two masses that are compared lie within 2^-40 of their size (C > 512 with top_p < 1: C^2 2^-62) of each
+ * other; the logarithm is that of a sum in float32 where C <= 512, off by up to (1.2 C + 30) 2^-24 besides its own rounding
+ * (typically by 2^-22), and in float64 beyond.
  * temperature <= 0 or NaN, top_p <= 0 or NaN, min_p > 1 or NaN: the first class of the order, logarithm 0.  NaN logits count as -inf;
  * a row without a class above -inf and rows behind T_len give -1 and 0.  The *_B arrays ([B], device) override the numbers where
  * not NULL.  C <= 524288. */

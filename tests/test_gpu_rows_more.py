@@ -59,3 +59,56 @@ def test_rows_with_infinities_and_nan_have_no_statistics():
     bad = torch.tensor([False, True, True, True, False, False], device="cuda")
     assert torch.isnan(y[bad]).all() and torch.isnan(rstd[bad]).all() and not torch.isfinite(mean[bad]).any()
     assert torch.isfinite(y[~bad]).all() and torch.isfinite(rstd[~bad]).all()
+
+
+# ---- sample_labels: many borders close together ------------------------------------------------------------------------------
+
+def drawn_in_order(z, u, p):
+    """labels of rows [R, C] by the definition in 64 bits (temperature 1), and the nearest that any comparison came to a tie, relative
+    to the mass"""
+    R, C = z.shape
+    v, order = torch.sort(z, dim=1, descending=True, stable=True)
+    w = torch.exp(v - v[:, :1])
+    run = w.cumsum(1)
+    front, target = run - w, p * run[:, -1:]
+    keep = front < target
+    keep[:, 0] = True
+    near = ((front - target).abs() / run[:, -1:]).min(1).values
+    kept = torch.zeros_like(w).scatter_(1, order, w * keep)
+    mass = kept.cumsum(1)
+    goal = u[:, None] * mass[:, -1:]
+    label = (mass > goal).int().argmax(1)
+    near = torch.minimum(near, ((mass - goal).abs() / mass[:, -1:]).min(1).values)
+    return label.int(), near
+
+
+@pytest.mark.parametrize("C", [5, 20, 67, 80, 81, 250, 320, 321, 512])
+@pytest.mark.parametrize("step", [1e-6, 1e-4, 1e-2, 1.0])
+def test_classes_a_hair_apart(C, step):
+    """Logits `step` apart in shuffled order: the halvings of the range of values leave up to all classes to walk past one by one, and
+    neighbouring borders are 1 / C of the mass apart.  Labels are whole numbers: equal wherever 64 bits decide (2^-40 of the mass)."""
+    g = torch.Generator().manual_seed(C)
+    R = 3000
+    z = torch.stack([torch.randperm(C, generator=g) for _ in range(R)]).float() * step
+    u, p = torch.rand(R, generator=g), torch.rand(R, generator=g) * 0.998 + 0.001
+    want, near = drawn_in_order(z.double(), u.double(), p.double()[:, None])
+    got, logp = bfa.sample_labels(z.reshape(R, 1, C).cuda(), u.reshape(R, 1).cuda(), top_p=p.cuda())
+    sure = near > 2.0 ** -40
+    assert sure.float().mean() > 0.99
+    assert torch.equal(got[:, 0].cpu()[sure], want[sure])
+
+
+def test_numbers_at_the_borders():
+    """numbers a few steps of float32 on either side of every border between the classes of a row, even and uneven"""
+    for C in (17, 67, 80, 300, 512):
+        g = torch.Generator().manual_seed(C + 1)
+        row = torch.randn(C, generator=g) * 2
+        for z in (row, torch.zeros(C)):
+            w = torch.exp(z.double() - z.double().max())
+            edge = (w.cumsum(0) / w.sum())[:-1].float()
+            u = torch.cat([edge] + [torch.nextafter(edge, torch.full_like(edge, s)) for s in (0.0, 1.0)]).clamp(0, 1 - 2.0 ** -24)
+            rows_in = z.expand(u.numel(), C).contiguous()
+            want, near = drawn_in_order(rows_in.double(), u.double(), torch.full((u.numel(), 1), 2.0, dtype=torch.float64))
+            got = bfa.sample_labels(rows_in.reshape(-1, 1, C).cuda(), u.reshape(-1, 1).cuda())[0][:, 0].cpu()
+            sure = near > 2.0 ** -40
+            assert torch.equal(got[sure], want[sure])
