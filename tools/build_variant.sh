@@ -6,7 +6,7 @@ set -e
 NAME=$1; UNIT=$2; shift 2
 CS=$(dirname "$0")/../bournemouth-forced-aligner_amd/csrc
 mkdir -p $CS/../variants
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -fno-slp-vectorize -Wall -Wno-unused-function"
+F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -fno-slp-vectorize -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
 /opt/rocm/bin/hipcc $F "$@" -c $CS/$UNIT.hip -o /tmp/variant_$NAME.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $CS/../variants/libbfa_$NAME.so $(ls $CS/build/*.o | grep -v "/$UNIT.hip.o") /tmp/variant_$NAME.o
 echo "built $CS/../variants/libbfa_$NAME.so"

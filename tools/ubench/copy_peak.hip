@@ -1,5 +1,5 @@
 // tools/ubench/copy_peak.hip -- which float4 copy kernel reaches the copy ceiling of the box (bfa_profile_copy uses the winner).
-// hipcc --offload-arch=gfx950 -O3 -o /tmp/copy_peak tools/ubench/copy_peak.hip && /tmp/copy_peak
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/copy_peak tools/ubench/copy_peak.hip && /tmp/copy_peak
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

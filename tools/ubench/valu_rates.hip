@@ -1,5 +1,6 @@
 // tools/ubench/valu_rates.hip -- measured issue cost (cycles per wave64 instruction per SIMD) of the VALU
-// instructions K1 is made of, on the GPU it runs on.  hipcc --offload-arch=gfx950 -O3 valu_rates.hip -o valu_rates
+// instructions K1 is made of, on the GPU it runs on.  hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops
+// valu_rates.hip -o valu_rates (packed float32 instructions are not used anywhere here: some of their forms have given wrong results)
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
@@ -20,11 +21,6 @@ __global__ __launch_bounds__(256) void k(float *out, int n)
             asm volatile("v_fma_f32 %0, %0, %8, %9\n v_fma_f32 %1, %1, %8, %9\n v_fma_f32 %2, %2, %8, %9\n v_fma_f32 %3, %3, %8, %9\n"
                          "v_fma_f32 %4, %4, %8, %9\n v_fma_f32 %5, %5, %8, %9\n v_fma_f32 %6, %6, %8, %9\n v_fma_f32 %7, %7, %8, %9\n"
                          : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7) : "v"(b), "v"(c));
-        } else if (KIND == 1) { // v_pk_fma_f32 (4 instr on pairs)
-            asm volatile("v_pk_fma_f32 %0, %0, %4, %5\n v_pk_fma_f32 %1, %1, %4, %5\n v_pk_fma_f32 %2, %2, %4, %5\n v_pk_fma_f32 %3, %3, %4, %5\n"
-                         "v_pk_fma_f32 %0, %0, %4, %5\n v_pk_fma_f32 %1, %1, %4, %5\n v_pk_fma_f32 %2, %2, %4, %5\n v_pk_fma_f32 %3, %3, %4, %5\n"
-                         : "+v"(*(double *)&a0), "+v"(*(double *)&a2), "+v"(*(double *)&a4), "+v"(*(double *)&a6)
-                         : "v"(*(double *)&b), "v"(*(double *)&c));
         } else if (KIND == 2) { // v_add_f32
             asm volatile(REP8("v_add_f32 %0, %0, %2\n v_add_f32 %1, %1, %2\n") "" : "+v"(a0), "+v"(a1) : "v"(b));
         } else if (KIND == 3) { // v_max3_f32
@@ -53,10 +49,6 @@ __global__ __launch_bounds__(256) void k(float *out, int n)
                          "v_mov_b32_dpp %0, %4 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:1\n v_mov_b32_dpp %1, %5 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:1\n"
                          "v_mov_b32_dpp %2, %6 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:1\n v_mov_b32_dpp %3, %7 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:1\n"
                          : "=v"(a0), "=v"(a1), "=v"(a2), "=v"(a3) : "v"(a4), "v"(a5), "v"(a6), "v"(a7));
-        } else if (KIND == 9) { // v_pk_add_f32
-            asm volatile("v_pk_add_f32 %0, %0, %4\n v_pk_add_f32 %1, %1, %4\n v_pk_add_f32 %2, %2, %4\n v_pk_add_f32 %3, %3, %4\n"
-                         "v_pk_add_f32 %0, %0, %4\n v_pk_add_f32 %1, %1, %4\n v_pk_add_f32 %2, %2, %4\n v_pk_add_f32 %3, %3, %4\n"
-                         : "+v"(*(double *)&a0), "+v"(*(double *)&a2), "+v"(*(double *)&a4), "+v"(*(double *)&a6) : "v"(*(double *)&b));
         } else if (KIND == 10) { // v_readlane_b32
             unsigned s0, s1, s2, s3;
             asm volatile("v_readlane_b32 %0, %4, 0\n v_readlane_b32 %1, %5, 1\n v_readlane_b32 %2, %6, 2\n v_readlane_b32 %3, %7, 3\n"
@@ -108,7 +100,6 @@ int main()
 {
     for (int w : {1, 2, 4, 8}) {
         run<0>("v_fma_f32", 8, w);
-        run<1>("v_pk_fma_f32", 8, w);
         run<2>("v_add_f32 (dep pairs)", 16, w);
         run<3>("v_max3_f32", 8, w);
         run<4>("v_cndmask (sgpr mask)", 8, w);
@@ -116,7 +107,6 @@ int main()
         run<6>("v_rndne+v_cvt_i32", 8, w);
         run<7>("v_cmp_lt+v_addc", 8, w);
         run<8>("v_mov_dpp", 8, w);
-        run<9>("v_pk_add_f32", 8, w);
         run<10>("v_readlane_b32", 8, w);
         run<11>("v_fma_f64", 16, w);
         run<12>("s_lshl/lshr_b64", 16, w);
