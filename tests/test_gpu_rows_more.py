@@ -112,3 +112,112 @@ def test_numbers_at_the_borders():
             got = bfa.sample_labels(rows_in.reshape(-1, 1, C).cuda(), u.reshape(-1, 1).cuda())[0][:, 0].cpu()
             sure = near > 2.0 ** -40
             assert torch.equal(got[sure], want[sure])
+
+
+# ---- more rows than the workgroups of a launch take at a time ----------------------------------------------------------------
+
+def ragged(B, T, seed):
+    """lengths, and which rows they hold"""
+    lengths = torch.randint(T // 2, T + 1, (B,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32)
+    lengths[0] = T
+    return lengths.cuda(), (torch.arange(T)[None] < lengths[:, None]).cuda()
+
+
+def rows_64(B, T, C, dtype, seed, scale=1.0, shift=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(B, T, C, generator=g, device="cuda") * scale + shift).to(dtype)
+    return x, x.double()
+
+
+# rows of 16, 64, 256 and 1024 threads, 16 / 4 / 1 / 1 rows to a workgroup of up to 2048 (backward 1024; 512 of 1024 threads), and swept
+# rows of up to 512 workgroups, 64 of column sums
+NORM_MANY = [(8, 5000, 33), (4, 2500, 300), (3, 900, 1100), (2, 320, 4200), (2, 300, 16400)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("shape", NORM_MANY, ids=lambda s: "x".join(map(str, s)))
+def test_layer_norm_of_many_rows(shape, dtype):
+    """Statistics as in test_far_means; the backward pass takes mean and rstd as float32.  Sums over rows: rows / 512 in a thread at
+    most, 16 in a workgroup, then 64 + 16 of partial sums."""
+    B, T, C = shape
+    lengths, held = ragged(B, T, 5)
+    x, xd = rows_64(B, T, C, dtype, 1, 1.5, 0.5)
+    gy, gd = rows_64(B, T, C, dtype, 2)
+    w = (1 + 0.2 * torch.randn(C, generator=torch.Generator().manual_seed(3))).to(dtype).cuda().requires_grad_()
+    b = (0.2 * torch.randn(C, generator=torch.Generator().manual_seed(4))).to(dtype).cuda().requires_grad_()
+    x.requires_grad_()
+    y = bfa.layer_norm(x, w, b, lengths=lengths)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), gy)
+    h, wd, bd, rows_held = half_step(dtype), w.detach().double(), b.detach().double(), held[..., None]
+    mean = xd.mean(-1, keepdim=True)
+    r = 1 / torch.sqrt(((xd - mean) ** 2).mean(-1, keepdim=True) + float(torch.tensor(1e-5)))
+    xh = (xd - mean) * r
+    want = (xh * wd + bd) * rows_held
+    tol = (64 * E + 40 * E * xh.abs()) * wd.abs() + (h + E) * want.abs()
+    assert ((y.detach().double() - want).abs() <= tol).all() and (y.detach()[~held] == 0).all()
+    off = E * (mean * r).abs() + 30 * E * xh.abs() + E * (1 + xh.abs())  # of xh: the mean's rounding, rstd, two operations
+    g = gd * wd
+    g1, g2 = g.abs().mean(-1, keepdim=True), (g * xh).abs().mean(-1, keepdim=True)
+    want = r * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True)) * rows_held
+    far = off.amax(-1, keepdim=True)
+    tol = (h + 32 * E) * want.abs() + r * (4 * E * g.abs() + 60 * E * g1 + (60 * E * g2 + g1 * far) * xh.abs() + off * g2 + 4 * E * xh.abs() * g2)
+    assert ((dx.double() - want).abs() <= tol * rows_held + 1e-30).all() and (dx[~held] == 0).all()
+    depth = E * (B * T / 512 + 128)
+    gh = gd.abs() * rows_held
+    want = (gd * xh * rows_held).sum((0, 1))
+    assert ((dw.double() - want).abs() <= h * want.abs() + (gh * (depth * xh.abs() + off)).sum((0, 1))).all()
+    want = (gd * rows_held).sum((0, 1))
+    assert ((db.double() - want).abs() <= h * want.abs() + depth * gh.sum((0, 1))).all()
+
+
+# rows of 4, 16 and 64 lanes (64 / 16 / 4 to each of 2048 workgroups), then of 64, 256 and 1024 threads (4 / 1 / 1 to 2048 / 2048 / 512);
+# the last: more rows than 256 workgroups add weights of at a time
+LOSS_MANY = [(8, 17000, 17), (5, 7000, 67), (3, 3000, 300), (3, 3000, 600), (3, 800, 1100), (2, 300, 4200), (16, 66000, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=ids)
+@pytest.mark.parametrize("shape", LOSS_MANY, ids=lambda s: "x".join(map(str, s)))
+def test_label_loss_of_many_rows(shape, dtype):
+    """A row's exponentials are off by a few E, their sum by log2(C) + 16 additions more, its logarithm and the differences by E of their
+    magnitudes; the sums over rows are float64."""
+    B, T, C = shape
+    lengths, held = ragged(B, T, 6)
+    z, zd = rows_64(B, T, C, dtype, 7, 2.0)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    labels = torch.randint(-1, C, (B, T), generator=g, device="cuda", dtype=torch.int32)
+    weights = torch.rand(B, T, generator=g, device="cuda")
+    counts = held & (labels >= 0)
+    wt = weights.double() * counts
+    p = torch.softmax(zd, -1)
+    at = labels.clamp(min=0).long()[..., None]
+    nll = (torch.logsumexp(zd, -1) - zd.gather(-1, at)[..., 0]) * wt
+    loss, grad = bfa.label_loss_and_grad(z, labels, weights=weights, lengths=lengths)
+    deep = math.log2(C) + 32
+    mag = zd.abs().amax(-1) + math.log(C) + 1
+    total = wt.sum()
+    want = nll.sum() / total
+    assert abs(float(loss) - float(want)) <= float(E * (deep * mag * wt).sum() / total) + 4 * E * float(want)
+    one = torch.zeros_like(p).scatter_(-1, at, 1.0)
+    want = (p - one) * (wt / total)[..., None]
+    tol = half_step(dtype) * want.abs() + E * (wt / total)[..., None] * (p * (deep + 4 * mag[..., None]) + 4)
+    tol = tol + (2.0 ** -25 if dtype == torch.float16 else 1e-38)  # (half of float16's smallest step)
+    assert ((grad.double() - want).abs() <= tol).all() and (grad[~counts] == 0).all()
+    each = bfa.label_loss(z, labels, weights=weights, lengths=lengths, reduction="none")
+    assert ((each.double() - nll).abs() <= E * deep * mag * wt).all()
+
+
+# rows of 4, 16 and 64 lanes (64 / 16 / 4 to each of 8192 workgroups), and a workgroup of 1024 to each of them
+@pytest.mark.parametrize("shape", [(8, 70000, 17), (4, 34000, 100), (3, 11500, 400), (2, 600, 600)], ids=lambda s: "x".join(map(str, s)))
+def test_sample_labels_of_many_rows(shape):
+    B, T, C = shape
+    lengths, held = ragged(B, T, 9)
+    z, zd = rows_64(B, T, C, torch.float32, 10, 2.0)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    u = torch.rand(B, T, generator=g, device="cuda")
+    p = torch.rand(B, generator=g, device="cuda") * 0.9 + 0.05
+    got, logp = bfa.sample_labels(z, u, top_p=p, lengths=lengths)
+    want, near = drawn_in_order(zd.reshape(-1, C), u.reshape(-1).double(), p.double()[:, None].expand(B, T).reshape(-1, 1))
+    sure = held & (near.reshape(B, T) > 2.0 ** -40)
+    assert float(sure.sum() / held.sum()) > 0.999
+    assert torch.equal(got[sure], want.reshape(B, T)[sure])
+    assert (got[~held] == -1).all() and (logp[~held] == 0).all()
