@@ -14,9 +14,11 @@
 // of its own columns in registers.  Per workgroup one partial sum per column goes to the workspace, and k_norm_cols adds those
 // in a fixed order: no atomics, the same bits every time.
 //
-// Measured: 32768 rows of 4096 bfloat16 channels 104 us forward (5.2 TB/s; 100 without the correction of the mean), 168 us backward
-// (4.8 TB/s) + 6.5 for the column sums; 16 ragged utterances of up to 1870 x 768 float32 24 + 35 + 5 us; 12000 ragged rows of 1001
+// Measured: 32768 rows of 4096 bfloat16 channels 104-107 us forward (5.0-5.2 TB/s; 100 without the correction of the mean), 171 us
+// backward (4.7 TB/s) + 6.6 for the column sums; 16 ragged utterances of up to 1870 x 768 float32 24 + 35 + 5 us; 12000 ragged rows of 1001
 // float16 channels, every row at another alignment, 11 + 15 + 6 us (35 + 21 with the weights loaded one by one).
+// 8192 rows of 8192 / 16384 bfloat16 channels 60 / 122-126 us forward (4.5 / 4.4 TB/s), 122 + 7 / 203 + 14 us backward (3.3 / 4.0 TB/s:
+// x, dy, w and the two sums as floats, 7 to 16 vector registers spilled); of 20480, swept element by element, 430 us and 662 + 266 + 6 us.
 #include <algorithm>
 
 #include "bfa_rows.hpp"

@@ -290,8 +290,9 @@ __device__ __forceinline__ bool draw_fast(const float (&z)[E], int at, int C, fl
 
 // Short rows (C <= 512): G lanes share a row, each holds E consecutive classes.  Bound: instructions -- the draw in float32, with
 // the end of a prefix bracketed by halving, and float64 for the rows that float32 leaves undecided (about one in a thousand).
-// 4096 x 1000 rows of 67 float32 logits with top-p 0.79 ms (16 lanes to a row 1.27, everything in float64 and walking down from the
-// top 4.6); 300 x 1500 ragged rows of 17 float16 logits with top-k 22 us (37).
+// 4096 x 1000 rows of 67 float32 logits with top-p 0.73 ms (16 lanes to a row 1.27, everything in float64 and walking down from the
+// top 4.6); 300 x 1500 ragged rows of 17 float16 logits with top-k 21 us (37).  The former take 1474 vector instructions per
+// 16 rows: 0.61 ms at 4 cycles each.
 template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sample_short(SampleArgs a)
 {
     constexpr int RPG = 256 / G;
@@ -422,7 +423,7 @@ template <typename T, int G, int E> __global__ __launch_bounds__(256) void k_sam
 // Bound: the float64 exponentials of the histogram and of the draw where k does not bound the prefix, latency for few rows.  One
 // workgroup per CU (with two, 64 registers a thread, the float64 polynomial spills: 604 us instead of 235 at the time).
 // 512 rows of 131072 bfloat16 logits with parameters of their own 0.19 ms (searching every border bit by bit: 2.9), all with
-// k = 50 62 us, all with p = 0.9 0.3 ms; 8 rows of 32000 float32 logits 43 us (472).
+// k = 50 63 us, all with p = 0.9 0.33 ms; 8 rows of 32000 float32 logits 43 us (472).
 constexpr int SAMPLE_MAX_C = 1 << 19, SAMPLE_BLOCKS = SAMPLE_MAX_C / (64 * 4);
 constexpr int SAMPLE_LIST = 2048, SAMPLE_LIST_K = 224, SAMPLE_BINS = 2048;
 
